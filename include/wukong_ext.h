@@ -114,6 +114,76 @@ int wk_attention_decode(void *out, const void *q, const void *kpool, const void 
                         int max_pages, const int *seq, const int *pos, int rows, int max_len, int n_heads,
                         int kv_heads, int head_dim, int dtype);
 
+/* ---- Continuous batching over an 8-bit paged K/V cache (no counterpart in
+ * the reference, which has no cache).  One step of a serving loop: wk_batch_plan
+ * (the maps of the step), wk_attention_packed (prompts) or wk_kv8_attention
+ * (single tokens), wk_kv8_store (append).  All run on the library stream, do not
+ * synchronise, allocate nothing and may be captured into a graph.  Each returns 0,
+ * or -1 with the reason in wk_last_error() and nothing launched.
+ *
+ * The cache: kpool / vpool [n_pages][kv_heads][64][head_dim] e4m3 codes (16-byte
+ * aligned) and kscale / vscale [n_pages][kv_heads] fp32; a value is code * scale.
+ * Sequence i's token p lies in page block_table[i][p / 64] at place p % 64.  A
+ * page id outside [0, n_pages) stands for no page: a token stored there is
+ * dropped, a key there is not attended to. */
+
+/* The maps of one step, from request lengths: sequence i (0 <= i < n <= 8192)
+ * has ctx[i] tokens in the cache and brings add[i] (0: none) more.  Device
+ * arrays, negative lengths count as 0:
+ *   starts [n + 1]  first packed row of each sequence; starts[n] is the row count
+ *   lens [n]        ctx + add, the next step's ctx (not the same array as ctx)
+ *   row_seq, row_pos [rows_cap], row_slot [rows_cap] (may be null)
+ *                   the sequence, position and cache slot 64 page + place of each
+ *                   row; -1 in the rows behind the last, and in row_slot where a
+ *                   row has no page
+ *   block_table [n][max_pages]  in and out: the entries of the ceil(ctx / 64) pages
+ *                   that a sequence holds are read, those of its new pages are
+ *                   written, the others are left alone
+ *   free_pages [free_cap], n_free [1]  page ids to hand out, from the front, in
+ *                   sequence order; where they run out, -1 is written
+ *   status [3]      rows, pages taken from free_pages, pages missing */
+int wk_batch_plan(int *starts, int *lens, int *row_seq, int *row_pos, long long *row_slot, int rows_cap,
+                  int *block_table, int max_pages, int *status, const int *ctx, const int *add, int n,
+                  const int *free_pages, const int *n_free, int free_cap);
+/* Append K and V rows (row r at k + r k_rs and v + r v_rs, strides in elements,
+ * [kv_heads][head_dim] of dtype F16 or BF16; head_dim 64 or 128): rows
+ * starts[i] .. starts[i+1] - 1 become the tokens ctx[i], ctx[i] + 1, ... of
+ * sequence i.  The scale of a page and head is the smallest power of two s
+ * with |x| <= 448 s over the tokens written to it (2^-100 if all are 0); codes are
+ * x / s rounded to nearest even.  When new tokens outgrow the scale of a page that
+ * already holds tokens, those are rounded again at the new scale.  Infinities
+ * saturate, NaN stays NaN, neither counts for the scale.  A page that the call
+ * writes must belong to one sequence only. rows bounds starts; rows behind
+ * starts[n] are not read. */
+int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_pages, const void *k, long k_rs,
+                 const void *v, long v_rs, const int *starts, const int *ctx, int n, int rows, const int *block_table,
+                 int max_pages, int kv_heads, int head_dim, int dtype);
+/* wk_attention_decode over that cache: row r is a token of sequence seq[r] at
+ * position pos[r] and sees the keys 0 .. pos[r]; a row whose seq is outside
+ * [0, n_seqs), or whose pos is negative, gets zeros.  Several rows may share a
+ * sequence.  n_heads a multiple of kv_heads; head_dim 64 or 128; dtype of q and
+ * out F16 or BF16; strides in elements.  max_len (the longest pos + 1) only
+ * chooses how the work is split.  ws [ws_bytes] is the caller's workspace (16-byte
+ * aligned), held until the call has run: calls that may overlap need one each;
+ * wk_kv8_attention_ws gives the bytes that the best split takes, with fewer (or
+ * null and 0) the context is split less. */
+long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim);
+int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
+                     const float *kscale, const float *vscale, int n_pages, const int *block_table, int n_seqs,
+                     int max_pages, const int *seq, const int *pos, int rows, int max_len, int n_heads, int kv_heads,
+                     int head_dim, int dtype, void *ws, long long ws_bytes);
+/* Causal attention over packed sequences: sequence i has the query rows
+ * q_starts[i] .. q_starts[i+1] - 1 and the key rows k_starts[i] .. k_starts[i+1] - 1
+ * (device int [n + 1], ascending), and its queries are the last of its keys: query j
+ * of Lq sees keys 0 .. Lk - Lq + j of its own sequence; one that sees none gets
+ * zeros.  Rows outside every sequence are neither read nor written.  q / out
+ * [q_rows][n_heads][head_dim], k / v [k_rows][kv_heads][head_dim] with row strides in
+ * elements (the slices of fused q|k|v rows serve); n_heads a multiple of kv_heads,
+ * head_dim 64 or 128, dtype F16 or BF16. */
+int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const void *k, long k_rs, const void *v,
+                        long v_rs, const int *q_starts, const int *k_starts, int n, int q_rows, int k_rows,
+                        int n_heads, int kv_heads, int head_dim, int dtype);
+
 /* Synthetic weights, bit-identical to the CPU oracle's generator:
  * Irwin-Hall(4) normal(0, stdv) samples of a counter-based hash. */
 int wk_fill_random_q8_0(void *dst, long rows, int cols, uint64_t seed, float stdv);

@@ -306,6 +306,18 @@ template <typename T> int allreduce_resid(T *x, float *p, long n, cudaStream_t s
 // Records the message returned by wk_last_error() and returns -1.
 int fail(const char *fmt, ...);
 
+// Makes the library's device current for one entry point and puts the caller's back.
+struct DeviceGuard {
+    int prev = -1;
+    DeviceGuard() {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != g_rt.device) cudaSetDevice(g_rt.device);
+    }
+    ~DeviceGuard() {
+        if (prev >= 0 && prev != g_rt.device) cudaSetDevice(prev);
+    }
+};
+
 // ---------------------------------------------------------------- layers.cu
 void layers_init();
 void layers_fini();
