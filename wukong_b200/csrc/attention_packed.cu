@@ -4,6 +4,8 @@
 // [k_starts[i], k_starts[i+1]); its queries are the last of its keys, so query
 // row j of Lq sees the keys 0 .. Lk - Lq + j:
 //   o = sum_k softmax_k(q . k / sqrt(d)) v
+#include <cudaTypedefs.h>
+
 #include "common.cuh"
 #include "wukong_ext.h"
 #include "wukong_internal.cuh"
@@ -80,6 +82,579 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
         reinterpret_cast<T *>(a.out)[row * a.out_rs + h * D + tid] = from_float<T>(l > 0.f || l != l ? o / l : 0.f);
 }
 
+// ------------------------------------------------------------------ tcgen05 kernel
+// A CTA takes one unit: 2 tiles of 128 query rows of one K/V head, a tile being
+// PT = 128 / G positions times the G heads of the group (heads inner), so that a
+// K/V tile loaded once serves all of them.  Per block of 128 keys and tile t:
+//   S_t = Q_t K^T  (TMEM, fp32)       P_t = exp2(c (S_t - m))  (16 bits, over S_t in TMEM)
+//   O_t += P_t V   (TMEM, fp32)       l_t += row sums of P_t before rounding
+// m is a maximum that is moved, and O_t and l_t scaled, only when it falls more
+// than 2^8 behind the running maximum: p <= 2^8 keeps its relative rounding, and
+// nearly every block skips the pass over O_t.
+//   warps 0-3, 4-7   softmax of tile 0, tile 1 (one thread per row), epilogue
+//   warp 8           issues the tcgen05.mma
+//   warp 9           TMA: Q, then K and V blocks through a ring
+//   warps 10, 11     clear what masked keys of V hold (see below)
+// While one tile's softmax runs on the CUDA cores, the tensor cores run the
+// other tile's P V and its next Q K^T.
+//
+// A masked key has p = 0, but 0 * NaN is NaN in a product of tiles.  So in the
+// blocks that some row of the unit sees in part, warps 10 and 11 set the rows of
+// V behind the sequence's end to zero, and every infinity or NaN inside it too,
+// noting its key and dimension; rows that do see that key get NaN there.
+constexpr int kPkThreads = 384;
+constexpr int kPkRegs = 168;  // registers per thread at launch
+constexpr int kPkKeys = 128;  // keys per block
+
+template <int D> struct PkLayout {
+    static constexpr int kTile = 128 * D * 2;                 // bytes of a Q tile or a K / V block
+    static constexpr int kStages = D == 128 ? 5 : 8;
+    static constexpr size_t kQ = 0;
+    static constexpr size_t kRing = 2 * (size_t)kTile;
+    static constexpr size_t kBars = kRing + (size_t)kStages * kTile;
+};
+
+template <int D> struct PkBars {
+    uint64_t q_full, kv_full[PkLayout<D>::kStages], kv_empty[PkLayout<D>::kStages];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t v_raw[4], v_clean[4];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
+    uint32_t tmem;
+    int found[4];      // sequence, unit within it
+    int units[12];
+    int bad;           // a non-finite V in a masked block
+    int bad_key[D];    // first key that holds one, per dimension
+};
+
+struct PkMaps {
+    CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ void pk_tma3(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void pk_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void pk_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void pk_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pk_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void pk_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void pk_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+#define WK_R32(v, o)                                                                                                 \
+    "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]),       \
+        "=r"(v[o + 7]), "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]),            \
+        "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]),         \
+        "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), "=r"(v[o + 24]),         \
+        "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]),         \
+        "=r"(v[o + 31])
+#define WK_I32(v, o)                                                                                                 \
+    "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]),              \
+        "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]), "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]),                  \
+        "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]),               \
+        "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]),               \
+        "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]), "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]),               \
+        "r"(v[o + 31])
+// 32 columns of this warp's 32 TMEM lanes, one lane per thread (no wait)
+__device__ __forceinline__ void pk_ld(uint32_t taddr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : WK_R32(v, 0)
+        : "r"(taddr));
+}
+__device__ __forceinline__ void pk_st(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        WK_I32(v, 0)
+        : "memory");
+}
+__device__ __forceinline__ void pk_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pk_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float pk_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// shared-memory descriptors, 128-byte swizzle: K-major rows of 128 bytes (8-row
+// groups 1024 bytes apart), and MN-major (the contraction runs over the rows;
+// 64-element column blocks `lbo` bytes apart)
+__device__ __forceinline__ uint64_t pk_desc(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <typename T> struct PkType {
+    static constexpr uint32_t fmt = 0;                  // kind::f16 operand format: f16
+    static constexpr uint32_t exp_one = 0x04000400u;    // one unit of the exponent field, both halves
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&h);
+    }
+};
+template <> struct PkType<__nv_bfloat16> {
+    static constexpr uint32_t fmt = 1;
+    static constexpr uint32_t exp_one = 0x00800080u;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&h);
+    }
+};
+
+struct PkArgs {
+    void *out;
+    long out_rs;
+    const int *q_starts, *k_starts;
+    int n, q_rows, k_rows, G, GT, chunks, kv_heads;  // heads per K/V head, heads per tile, tiles of heads per K/V head
+    float scale_log2;
+    int vec;  // out is 16-byte aligned and strided
+    int *err;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPkThreads, 1)
+    attn_packed_kernel(const __grid_constant__ PkMaps maps, const PkArgs a) {
+    using L = PkLayout<D>;
+    constexpr int ST = L::kStages;
+    extern __shared__ __align__(1024) uint8_t pk_smem[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)pk_smem + 1023) & ~(uintptr_t)1023);
+    PkBars<D> *B = reinterpret_cast<PkBars<D> *>(smem + L::kBars);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        mbar_init(&B->q_full, 1);
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&B->kv_full[i], 1);
+            mbar_init(&B->kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B->s_full[i], 1);
+            mbar_init(&B->p_full[i], 128);
+            mbar_init(&B->o_full[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&B->v_raw[i], 1);
+            mbar_init(&B->v_clean[i], 64);
+        }
+        mbar_fence_init();
+        B->found[0] = -1;
+        B->bad = 0;
+    }
+    for (int i = tid; i < D; i += kPkThreads) B->bad_key[i] = 0x7fffffff;
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pk_fence_before();
+    pdl_wait();
+    pdl_trigger();
+    // ---- this CTA's unit: the idx-th from the end, so that the longest rows of a long prompt start first
+    const int hb = blockIdx.x % (a.kv_heads * a.chunks), idx = blockIdx.x / (a.kv_heads * a.chunks);
+    const int kvh = hb / a.chunks, chunk = hb % a.chunks;
+    const int PT = 128 / a.GT;
+    int before = 0;
+    for (int i0 = 0; i0 < a.n; i0 += kPkThreads) {
+        const int i = a.n - 1 - (i0 + tid);
+        int u = 0;
+        if (i >= 0) {
+            const int q0 = min(max(a.q_starts[i], 0), a.q_rows);
+            u = (min(max(a.q_starts[i + 1], q0), a.q_rows) - q0 + 2 * PT - 1) / (2 * PT);
+        }
+        int in = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, in, o);
+            if (lane >= o) in += v;
+        }
+        __syncthreads();
+        if (lane == 31) B->units[warp] = in;
+        __syncthreads();
+        int first = before + in - u;
+#pragma unroll
+        for (int w = 0; w < kPkThreads / 32; ++w) {
+            if (w < warp) first += B->units[w];
+            before += B->units[w];
+        }
+        if (idx >= first && idx < first + u) {
+            B->found[0] = i;
+            B->found[1] = u - 1 - (idx - first);
+        }
+        if (idx < before) break;
+    }
+    __syncthreads();
+    pk_fence_after();
+    const uint32_t tmem = B->tmem;
+    const int seq = B->found[0];
+    bool ok = true;
+    if (seq >= 0) {
+        const int q0 = min(max(a.q_starts[seq], 0), a.q_rows);
+        const int ql = min(max(a.q_starts[seq + 1], q0), a.q_rows) - q0;
+        const int k0 = min(max(a.k_starts[seq], 0), a.k_rows);
+        const int kl = min(max(a.k_starts[seq + 1], k0), a.k_rows) - k0;
+        const int shift = kl - ql;                // query j sees keys 0 .. shift + j
+        const int j0 = B->found[1] * 2 * PT;      // first query of the unit
+        const int head0 = kvh * a.G + chunk * a.GT;
+        // blocks of keys that each tile sees (0: none), and the first that some row of the unit sees in part
+        auto blocks = [&](int t) -> int {
+            const int f = j0 + t * PT;
+            if (f >= ql) return 0;
+            const int last = shift + min(f + PT, ql) - 1;  // the last key that the tile sees
+            return last < 0 ? 0 : last / kPkKeys + 1;
+        };
+        const int n0 = blocks(0), n1 = blocks(1), nb = max(n0, n1);
+        const int part = max(0, (shift + j0 + 1) / kPkKeys);  // blocks below this are seen whole by every row
+        // registers: 2 softmax warpgroups x 128 x 216 + 128 x 72 = the launch's 384 x 168
+        if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 9) {
+            if (lane == 0 && nb > 0) {
+                const uint32_t qbytes = (uint32_t)(PT * a.GT) * D * 2;
+                auto load_q = [&](int t) {
+                    for (int b = 0; b < D / 64; ++b)
+                        pk_tma3(smem + L::kQ + t * L::kTile + b * 16384, &maps.q, 64 * b, head0, q0 + j0 + t * PT,
+                                &B->q_full);
+                };
+                mbar_expect_tx(&B->q_full, n1 > 0 ? 2 * qbytes : qbytes);
+                load_q(0);
+                auto raw = [&](int i) -> uint64_t * {
+                    return (i & 1) && (i >> 1) >= part ? &B->v_raw[((i >> 1) - part) & 3] : nullptr;
+                };
+                int issued = 0;
+                for (int i = 0; i < 2 * nb; ++i) {
+                    const int s = i % ST;
+                    if (i >= ST && !mbar_wait_bounded(&B->kv_empty[s], ((i / ST) - 1) & 1, a.err, 50)) {
+                        ok = false;
+                        break;
+                    }
+                    uint64_t *bar = &B->kv_full[s];
+                    if (raw(i)) {  // lands on a barrier of its own; the ring's only keeps step
+                        pk_arrive(bar);
+                        bar = raw(i);
+                    }
+                    mbar_expect_tx(bar, L::kTile);
+                    const CUtensorMap *m = (i & 1) ? &maps.v : &maps.k;
+                    for (int b = 0; b < D / 64; ++b)
+                        pk_tma3(smem + L::kRing + (size_t)s * L::kTile + b * 16384, m, 64 * b, kvh,
+                                k0 + (i >> 1) * kPkKeys, bar);
+                    ++issued;
+                    if (i == 0 && n1 > 0) load_q(1);
+                }
+                if (!ok)  // no copy of this CTA may land after it has left
+                    for (int i = max(0, issued - ST); i < issued; ++i) {
+                        if (raw(i))
+                            mbar_wait_bounded(raw(i), (((i >> 1) - part) >> 2) & 1, a.err, 51);
+                        else
+                            mbar_wait_bounded(&B->kv_full[i % ST], (i / ST) & 1, a.err, 51);
+                    }
+            }
+        } else if (warp == 8) {
+            if (lane == 0 && nb > 0) {
+                constexpr uint32_t fmt = (1u << 4) | (PkType<T>::fmt << 7) | (PkType<T>::fmt << 10) | (8u << 24);
+                constexpr uint32_t id_qk = fmt | (uint32_t)(kPkKeys >> 3) << 17;
+                constexpr uint32_t id_pv = fmt | (1u << 16) | (uint32_t)(D >> 3) << 17;  // B (V) MN-major
+                const uint32_t ring = smem_u32(smem + L::kRing), qs = smem_u32(smem + L::kQ);
+                auto wait_kv = [&](int i) {
+                    if (ok && !mbar_wait_bounded(&B->kv_full[i % ST], (i / ST) & 1, a.err, 52)) ok = false;
+                };
+                auto qk = [&](int t, int j) {
+                    const uint32_t kb = ring + ((2 * j) % ST) * L::kTile, qb = qs + t * L::kTile;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t o = (kk >> 2) * 16384 + (kk & 3) * 32;
+                        pk_mma_ss(tmem + t * 128, pk_desc(qb + o, 16), pk_desc(kb + o, 16), id_qk, kk != 0);
+                    }
+                    pk_commit(&B->s_full[t]);
+                };
+                auto pv = [&](int t, int j) {
+                    const uint32_t vb = ring + ((2 * j + 1) % ST) * L::kTile;
+#pragma unroll
+                    for (int kk = 0; kk < kPkKeys / 16; ++kk)
+                        pk_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * kk, pk_desc(vb + kk * 2048, 16384), id_pv,
+                                  (j | kk) != 0);
+                };
+                if (!mbar_wait_bounded(&B->q_full, 0, a.err, 53)) ok = false;
+                wait_kv(0);
+                if (ok) {
+                    pk_fence_after();
+                    if (n0 > 0) qk(0, 0);
+                    if (n1 > 0) qk(1, 0);
+                    pk_commit(&B->kv_empty[0]);
+                }
+                for (int j = 0; j < nb && ok; ++j) {
+                    wait_kv(2 * j + 1);
+                    if (j >= part && ok && !mbar_wait_bounded(&B->v_clean[(j - part) & 3], ((j - part) >> 2) & 1, a.err, 54))
+                        ok = false;
+                    if (j + 1 < nb) wait_kv(2 * j + 2);
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        const int nt = t ? n1 : n0;
+                        if (j < nt) {
+                            if (!mbar_wait_bounded(&B->p_full[t], j & 1, a.err, 55)) {
+                                ok = false;
+                                break;
+                            }
+                            pk_fence_after();
+                            pv(t, j);
+                            if (j + 1 == nt) pk_commit(&B->o_full[t]);
+                        }
+                        if (t == 1) pk_commit(&B->kv_empty[(2 * j + 1) % ST]);
+                        if (j + 1 < nt) qk(t, j + 1);
+                    }
+                    if (j + 1 < nb && ok) pk_commit(&B->kv_empty[(2 * j + 2) % ST]);
+                }
+            }
+        } else {
+            // ---- V of the blocks that are seen in part
+            const int ct = tid - 320;  // 0..63
+            for (int j = part; j < nb && ok; ++j) {
+                const int s = (2 * j + 1) % ST, c = j - part;
+                if (!mbar_wait_bounded(&B->v_raw[c & 3], (c >> 2) & 1, a.err, 56)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *vb = smem + L::kRing + (size_t)s * L::kTile;
+                const int live = min(kPkKeys, kl - j * kPkKeys);
+                // 16-byte chunks: chunk c of key row r lies at place c ^ (r & 7) of its 128 bytes
+                for (int q = ct; q < kPkKeys * D / 8; q += 64) {
+                    uint4 *p = reinterpret_cast<uint4 *>(vb) + q;
+                    const int r = (q >> 3) & 127;
+                    if (r >= live) {
+                        *p = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    const uint4 u = *p;
+                    const uint32_t e = PkType<T>::exp_one;
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    uint32_t hit = 0;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) hit |= (w[x] & 0x7fff7fffu) + e;
+                    if (hit & 0x80008000u) {
+                        const int d0 = (q >> 10) * 64 + ((q & 7) ^ (r & 7)) * 8;
+                        uint32_t z[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t over = ((w[x] & 0x7fff7fffu) + e) & 0x80008000u;
+                            z[x] = w[x];
+                            if (over & 0x8000u) {
+                                z[x] &= 0xffff0000u;
+                                atomicMin(&B->bad_key[d0 + 2 * x], j * kPkKeys + r);
+                            }
+                            if (over & 0x80000000u) {
+                                z[x] &= 0x0000ffffu;
+                                atomicMin(&B->bad_key[d0 + 2 * x + 1], j * kPkKeys + r);
+                            }
+                        }
+                        *p = make_uint4(z[0], z[1], z[2], z[3]);
+                        B->bad = 1;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                pk_arrive(&B->v_clean[c & 3]);
+            }
+        }
+        } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+            // ---- softmax: thread = row of tile t
+            const int t = warp >> 2, row = tid & 127;
+            const int nt = t ? n1 : n0;
+            const int jq = j0 + t * PT + row / a.GT;  // query of this row
+            const int lim = shift + jq;               // last key that it sees
+            const int lim0 = shift + j0 + t * PT;     // of the tile's first row
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+            const uint32_t s_t = tmem + t * 128 + lanes, o_t = tmem + 256 + t * 128 + lanes;
+            float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to
+            for (int j = 0; j < nt; ++j) {
+                // (the warp leaves as one: what follows is warp-wide)
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&B->s_full[t], j & 1, a.err, 57))) {
+                    ok = false;
+                    break;
+                }
+                pk_fence_after();
+                uint32_t sv[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) pk_ld(s_t + 32 * c, sv + 32 * c);
+                pk_wait_ld();
+                if (j * kPkKeys + kPkKeys - 1 > lim0) {
+                    const int seen = lim - j * kPkKeys;  // keys of the block up to this one
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (i > seen) sv[i] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(sv[i]);
+#pragma unroll
+                for (int i = 4; i < 128; i += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sv[i + e]));
+                const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool move = (mb - m) * a.scale_log2 > 8.f || (m == -INFINITY && mb > m);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float mn = move ? mb : m;
+                    const float f = mn == m || m == -INFINITY ? 1.f : pk_ex2((m - mn) * a.scale_log2);
+                    m = mn;
+                    l *= f;
+                    if (j > 0) {  // the products so far are complete: S of this block was issued after them
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t ov[32];
+                            pk_ld(o_t + 32 * c, ov);
+                            pk_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                            pk_st(o_t + 32 * c, ov);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pv[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float x = pk_ex2(fmaf(__uint_as_float(sv[64 * c + 2 * i]), a.scale_log2, base));
+                        const float y = pk_ex2(fmaf(__uint_as_float(sv[64 * c + 2 * i + 1]), a.scale_log2, base));
+                        sum[(2 * i) & 3] += x;
+                        sum[(2 * i + 1) & 3] += y;
+                        pv[i] = PkType<T>::pack(x, y);
+                    }
+                    pk_st(s_t + 32 * c, pv);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pk_wait_st();
+                pk_fence_before();
+                pk_arrive(&B->p_full[t]);
+            }
+            // ---- epilogue
+            if (nt > 0 && ok && !__all_sync(0xffffffffu, mbar_wait_bounded(&B->o_full[t], 0, a.err, 58))) ok = false;
+            pk_fence_after();
+            // what the clearing warps noted of this tile's blocks
+            if (nt > part && ok) mbar_wait_bounded(&B->v_clean[(nt - 1 - part) & 3], ((nt - 1 - part) >> 2) & 1, a.err, 59);
+            const int h = chunk * a.GT + row % a.GT;
+            const bool mine = row < PT * a.GT && jq < ql && h < a.G && ok;
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            const bool bad = nt > 0 && B->bad;
+            T *orow = reinterpret_cast<T *>(a.out) + (long)(q0 + jq) * a.out_rs + (long)(kvh * a.G + h) * D;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t ov[32];
+                if (nt > 0) {
+                    pk_ld(o_t + 32 * c, ov);
+                    pk_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) ov[i] = 0;
+                }
+                if (bad) {
+                    for (int i = 0; i < 32; ++i)
+                        if (B->bad_key[32 * c + i] <= lim) ov[i] = 0x7fc00000u;
+                }
+                if (mine) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = l == 0.f ? 0.f : __uint_as_float(ov[2 * i]) * inv;
+                        const float y = l == 0.f ? 0.f : __uint_as_float(ov[2 * i + 1]) * inv;
+                        w[i] = PkType<T>::pack(x, y);
+                    }
+                    if (a.vec) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            reinterpret_cast<uint4 *>(orow + 32 * c)[i] =
+                                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    } else {
+                        unsigned short *o = reinterpret_cast<unsigned short *>(orow + 32 * c);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            o[2 * i] = (unsigned short)w[i];
+                            o[2 * i + 1] = (unsigned short)(w[i] >> 16);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    pk_fence_before();
+    __syncthreads();
+    pk_fence_after();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// 3-D map over [rows][heads][D] 16-bit values with boxes of box_rows x box_heads x 64.
+bool pk_map(CUtensorMap *m, const void *base, int dtype, int D, int heads, int rows, long rs, int box_heads,
+            int box_rows) {
+    return encode_map_3d(m, base, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         D, heads, rows, 2 * (uint64_t)D, 2 * (uint64_t)rs, 64, box_heads, box_rows,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, const PkMaps &maps, int GT, cudaStream_t s) {
+    using L = PkLayout<D>;
+    const size_t smem = L::kBars + sizeof(PkBars<D>) + 1024;
+    auto kern = attn_packed_kernel<T, D>;
+    static bool configured = false;
+    if (!configured) {
+        cudaFuncAttributes fa;
+        cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+        if (e != cudaSuccess) return e;
+        if (fa.numRegs != kPkRegs) return cudaErrorInvalidKernelImage;  // the register split would not add up
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        configured = true;
+    }
+    PkArgs a;
+    a.out = p.out;
+    a.out_rs = p.out_rs;
+    a.q_starts = p.q_starts;
+    a.k_starts = p.k_starts;
+    a.n = p.n;
+    a.q_rows = p.q_rows;
+    a.k_rows = p.k_rows;
+    a.G = p.heads / p.kv_heads;
+    a.GT = GT;
+    a.chunks = (a.G + GT - 1) / GT;
+    a.kv_heads = p.kv_heads;
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.vec = ((uintptr_t)p.out % 16) == 0 && p.out_rs % 8 == 0;
+    a.err = g_rt.d_error;
+    const int PT = 128 / GT;
+    // units: ceil(length / (2 PT)) per sequence
+    const long long most = (long long)p.q_rows / (2 * PT) + p.n;
+    const long long units = most < p.q_rows ? most : p.q_rows;
+    if (units * p.kv_heads * a.chunks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * p.kv_heads * a.chunks));
+    cfg.blockDim = dim3(kPkThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_rt.pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, maps, a);
+}
+
 template <typename T, int D> cudaError_t launch_rows(const PackedArgs &a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.q_rows, a.heads);
@@ -121,7 +696,21 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
                  1.0f / sqrtf((float)head_dim)};
     cudaStream_t s = stream();
     cudaError_t e;
-    if (dtype == kF16)
+    // TMA wants 16-byte aligned bases and strides; what is not goes row by row
+    const uintptr_t low = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v;
+    if (low % 16 == 0 && (q_rs | k_rs | v_rs) % 8 == 0 && k_rows > 0) {
+        const int G = n_heads / kv_heads, GT = G < 128 ? G : 128;
+        PkMaps maps;
+        if (!pk_map(&maps.q, q, dtype, head_dim, n_heads, q_rows, q_rs, GT, 128 / GT) ||
+            !pk_map(&maps.k, k, dtype, head_dim, kv_heads, k_rows, k_rs, 1, kPkKeys) ||
+            !pk_map(&maps.v, v, dtype, head_dim, kv_heads, k_rows, v_rs, 1, kPkKeys))
+            return fail("wk_attention_packed: cuTensorMapEncodeTiled failed");
+        if (dtype == kF16)
+            e = head_dim == 64 ? launch_packed<__half, 64>(a, maps, GT, s) : launch_packed<__half, 128>(a, maps, GT, s);
+        else
+            e = head_dim == 64 ? launch_packed<__nv_bfloat16, 64>(a, maps, GT, s)
+                               : launch_packed<__nv_bfloat16, 128>(a, maps, GT, s);
+    } else if (dtype == kF16)
         e = head_dim == 64 ? launch_rows<__half, 64>(a, s) : launch_rows<__half, 128>(a, s);
     else
         e = head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(a, s) : launch_rows<__nv_bfloat16, 128>(a, s);

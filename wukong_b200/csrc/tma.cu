@@ -45,6 +45,18 @@ bool encode_map_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, uin
     return r == CUDA_SUCCESS;
 }
 
+bool encode_map_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, uint64_t d0, uint64_t d1, uint64_t d2,
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
+                   CUtensorMapSwizzle swizzle) {
+    cuuint64_t dims[3] = {d0, d1, d2};
+    cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
+    cuuint32_t box[3] = {box0, box1, box2};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = encoder()(m, dt, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
 const CUtensorMap *weight_map(const void *w, long rows, long row_bytes, int box_inner, int box_rows) {
     if (((uintptr_t)w % 16) || (row_bytes % 16) || rows <= 0) return nullptr;
     if (!g_maps) g_maps = (MapEntry *)calloc(kMapCache, sizeof(MapEntry));

@@ -11,6 +11,9 @@ namespace wk {
 // cudaGetDriverEntryPoint so that the library links without libcuda.
 bool encode_map_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, uint64_t inner, uint64_t outer,
                    uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
+bool encode_map_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, uint64_t d0, uint64_t d1, uint64_t d2,
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
+                   CUtensorMapSwizzle swizzle);
 // Cached map over a weight matrix viewed as [N rows][row_bytes / 2] uint16 with
 // boxes of `box_inner` uint16 x `box_rows` rows (null if the rows are not TMA-able).
 const CUtensorMap *weight_map(const void *w, long rows, long row_bytes, int box_inner, int box_rows);
