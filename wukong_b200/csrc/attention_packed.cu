@@ -145,6 +145,14 @@ __device__ __forceinline__ void pk_commit(uint64_t *bar) {
 }
 __device__ __forceinline__ void pk_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pk_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// One lane of a converged warp: unlike `lane == 0` it keeps the operands of what
+// follows in uniform registers, where tcgen05.mma takes them (with a plain lane
+// test a tile's 16 instructions took 1800 cycles to issue, more than they run).
+__device__ __forceinline__ bool pk_elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
 // D[tmem] (+)= A[smem] B[smem]
 __device__ __forceinline__ void pk_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -239,7 +247,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     extern __shared__ __align__(1024) uint8_t pk_smem[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)pk_smem + 1023) & ~(uintptr_t)1023);
     PkBars<D> *B = reinterpret_cast<PkBars<D> *>(smem + L::kBars);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in the whole warp
     if (tid == 0) {
         mbar_init(&B->q_full, 1);
         for (int i = 0; i < ST; ++i) {
@@ -327,7 +336,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 9) {
-            if (lane == 0 && nb > 0) {
+            if (nb > 0 && pk_elect()) {
                 const uint32_t qbytes = (uint32_t)(PT * a.GT) * D * 2;
                 auto load_q = [&](int t) {
                     for (int b = 0; b < D / 64; ++b)
@@ -368,7 +377,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
             }
         } else if (warp == 8) {
-            if (lane == 0 && nb > 0) {
+            if (nb > 0 && pk_elect()) {
                 constexpr uint32_t fmt = (1u << 4) | (PkType<T>::fmt << 7) | (PkType<T>::fmt << 10) | (8u << 24);
                 constexpr uint32_t id_qk = fmt | (uint32_t)(kPkKeys >> 3) << 17;
                 constexpr uint32_t id_pv = fmt | (1u << 16) | (uint32_t)(D >> 3) << 17;  // B (V) MN-major
