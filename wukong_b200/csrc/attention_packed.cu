@@ -116,7 +116,7 @@ template <int D> struct PkLayout {
 
 template <int D> struct PkBars {
     uint64_t q_full, kv_full[PkLayout<D>::kStages], kv_empty[PkLayout<D>::kStages];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
     uint64_t v_raw[4], v_clean[4];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
     uint32_t tmem;
     int found[4];      // sequence, unit within it
@@ -200,6 +200,37 @@ __device__ __forceinline__ void pk_st(uint32_t taddr, const uint32_t *v) {
 }
 __device__ __forceinline__ void pk_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pk_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// two fp32 values per instruction
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk_pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ f32x2 pk_pair(uint32_t lo, uint32_t hi) {
+    return pk_pair(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ float2 pk_unpair(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 pk_fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 pk_add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// the largest of three, NaN if one is
+__device__ __forceinline__ float pk_max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float pk_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -257,6 +288,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B->s_full[i], 1);
+            mbar_init(&B->p_half[i], 128);
             mbar_init(&B->p_full[i], 128);
             mbar_init(&B->o_full[i], 1);
         }
@@ -394,10 +426,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
                     pk_commit(&B->s_full[t]);
                 };
-                auto pv = [&](int t, int j) {
+                auto pv = [&](int t, int j, int half) {
                     const uint32_t vb = ring + ((2 * j + 1) % ST) * L::kTile;
 #pragma unroll
-                    for (int kk = 0; kk < kPkKeys / 16; ++kk)
+                    for (int kk = half * 4; kk < half * 4 + 4; ++kk)
                         pk_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * kk, pk_desc(vb + kk * 2048, 16384), id_pv,
                                   (j | kk) != 0);
                 };
@@ -417,12 +449,18 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     for (int t = 0; t < 2 && ok; ++t) {
                         const int nt = t ? n1 : n0;
                         if (j < nt) {
-                            if (!mbar_wait_bounded(&B->p_full[t], j & 1, a.err, 55)) {
+                            if (!mbar_wait_bounded(&B->p_half[t], j & 1, a.err, 55)) {
                                 ok = false;
                                 break;
                             }
                             pk_fence_after();
-                            pv(t, j);
+                            pv(t, j, 0);
+                            if (!mbar_wait_bounded(&B->p_full[t], j & 1, a.err, 60)) {
+                                ok = false;
+                                break;
+                            }
+                            pk_fence_after();
+                            pv(t, j, 1);
                             if (j + 1 == nt) pk_commit(&B->o_full[t]);
                         }
                         if (t == 1) pk_commit(&B->kv_empty[(2 * j + 1) % ST]);
@@ -508,14 +546,40 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     for (int i = 0; i < 128; ++i)
                         if (i > seen) sv[i] = 0xff800000u;
                 }
+                // exponentials of keys 64 c .. 64 c + 63, their sum and P
+                const f32x2 scale2 = pk_pair(a.scale_log2, a.scale_log2);
+                auto half = [&](int c, float m, f32x2(&sum)[2], uint32_t(&pv)[32]) {
+                    const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                    const f32x2 base2 = pk_pair(base, base);
+                    sum[0] = sum[1] = 0;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const f32x2 x = pk_fma2(pk_pair(sv[64 * c + 2 * i], sv[64 * c + 2 * i + 1]), scale2, base2);
+                        float2 u = pk_unpair(x);
+                        u.x = pk_ex2(u.x);
+                        u.y = pk_ex2(u.y);
+                        sum[i & 1] = pk_add2(sum[i & 1], pk_pair(u.x, u.y));
+                        pv[i] = PkType<T>::pack(u.x, u.y);
+                    }
+                };
+                // The first half is computed with the maximum so far while this block's is
+                // found (the exponentials and the maximum use different pipes), and again
+                // in the rare case that the maximum moves.
+                f32x2 sum[2];
+                uint32_t pv[32];
+                half(0, m, sum, pv);
                 float mx[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(sv[i]);
+                for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
 #pragma unroll
-                for (int i = 4; i < 128; i += 4)
+                for (int i = 4; i < 124; i += 8)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sv[i + e]));
-                const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int e = 0; e < 4; ++e)
+                        mx[e] = pk_max3(mx[e], __uint_as_float(sv[i + e]), __uint_as_float(sv[i + 4 + e]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = pk_max3(mx[e], __uint_as_float(sv[124 + e]), mx[e]);
+                const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+                if (mb != mb) l = mb;  // a key that this row sees scores NaN: so does the row
                 const bool move = (mb - m) * a.scale_log2 > 8.f || (m == -INFINITY && mb > m);
                 if (__any_sync(0xffffffffu, move)) {
                     const float mn = move ? mb : m;
@@ -533,26 +597,19 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                             pk_st(o_t + 32 * c, ov);
                         }
                     }
+                    half(0, m, sum, pv);
                 }
-                const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                // P goes to the tensor cores in two halves, the first while the second is computed
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t pv[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float x = pk_ex2(fmaf(__uint_as_float(sv[64 * c + 2 * i]), a.scale_log2, base));
-                        const float y = pk_ex2(fmaf(__uint_as_float(sv[64 * c + 2 * i + 1]), a.scale_log2, base));
-                        sum[(2 * i) & 3] += x;
-                        sum[(2 * i + 1) & 3] += y;
-                        pv[i] = PkType<T>::pack(x, y);
-                    }
+                    if (c) half(1, m, sum, pv);
+                    const float2 u = pk_unpair(pk_add2(sum[0], sum[1]));
+                    l += u.x + u.y;
                     pk_st(s_t + 32 * c, pv);
+                    pk_wait_st();
+                    pk_fence_before();
+                    pk_arrive(c ? &B->p_full[t] : &B->p_half[t]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                pk_wait_st();
-                pk_fence_before();
-                pk_arrive(&B->p_full[t]);
             }
             // ---- epilogue
             if (nt > 0 && ok && !__all_sync(0xffffffffu, mbar_wait_bounded(&B->o_full[t], 0, a.err, 58))) ok = false;
