@@ -120,7 +120,7 @@ template <int D> struct PkBars {
     uint64_t v_raw[4], v_clean[4];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
     uint32_t tmem;
     int found[4];      // sequence, unit within it
-    int units[12];
+    int units[kPkThreads / 32];
     int bad;           // a non-finite V in a masked block
     int bad_key[D];    // first key that holds one, per dimension
 };
@@ -135,6 +135,26 @@ __device__ __forceinline__ void pk_tma3(void *dst, const CUtensorMap *map, int x
             smem_u32(dst)),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
+}
+// Bounded wait as mbar_wait_bounded, with a short slow path: the waits of the
+// issuing warp run once per block of keys between two softmax warps whose code
+// fills the instruction cache, and every line of its own that it has to fetch
+// again costs more than the instructions in it.
+__device__ __forceinline__ bool pk_wait(uint64_t *bar, uint32_t parity, int *err, int code) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer_ns() - t0 > 1000000000ull) {
+            if (err) atomicCAS(err, 0, code);
+            return false;
+        }
+    return true;
+}
+__device__ __forceinline__ uint64_t pk_join(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
 }
 __device__ __forceinline__ void pk_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -364,7 +384,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         };
         const int n0 = blocks(0), n1 = blocks(1), nb = max(n0, n1);
         const int part = max(0, (shift + j0 + 1) / kPkKeys);  // blocks below this are seen whole by every row
-        // registers: 2 softmax warpgroups x 128 x 216 + 128 x 72 = the launch's 384 x 168
+        // registers: 256 softmax threads x 216 + 128 x 72 = the launch's 384 x 168
         if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 9) {
@@ -383,7 +403,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 int issued = 0;
                 for (int i = 0; i < 2 * nb; ++i) {
                     const int s = i % ST;
-                    if (i >= ST && !mbar_wait_bounded(&B->kv_empty[s], ((i / ST) - 1) & 1, a.err, 50)) {
+                    if (i >= ST && !pk_wait(&B->kv_empty[s], ((i / ST) - 1) & 1, a.err, 50)) {
                         ok = false;
                         break;
                     }
@@ -403,9 +423,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 if (!ok)  // no copy of this CTA may land after it has left
                     for (int i = max(0, issued - ST); i < issued; ++i) {
                         if (raw(i))
-                            mbar_wait_bounded(raw(i), (((i >> 1) - part) >> 2) & 1, a.err, 51);
+                            pk_wait(raw(i), (((i >> 1) - part) >> 2) & 1, a.err, 51);
                         else
-                            mbar_wait_bounded(&B->kv_full[i % ST], (i / ST) & 1, a.err, 51);
+                            pk_wait(&B->kv_full[i % ST], (i / ST) & 1, a.err, 51);
                     }
             }
         } else if (warp == 8) {
@@ -414,59 +434,75 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 constexpr uint32_t id_qk = fmt | (uint32_t)(kPkKeys >> 3) << 17;
                 constexpr uint32_t id_pv = fmt | (1u << 16) | (uint32_t)(D >> 3) << 17;  // B (V) MN-major
                 const uint32_t ring = smem_u32(smem + L::kRing), qs = smem_u32(smem + L::kQ);
-                auto wait_kv = [&](int i) {
-                    if (ok && !mbar_wait_bounded(&B->kv_full[i % ST], (i / ST) & 1, a.err, 52)) ok = false;
-                };
-                auto qk = [&](int t, int j) {
-                    const uint32_t kb = ring + ((2 * j) % ST) * L::kTile, qb = qs + t * L::kTile;
+                // the halves of a descriptor: the upper is constant, the lower the address
+                const uint32_t q_lo = (uint32_t)pk_desc(qs, 16), ring_lo = (uint32_t)pk_desc(ring, 16);
+                constexpr uint32_t hi = (uint32_t)(1024 >> 4) | 1u << 14 | 2u << 29;
+                constexpr uint32_t mn = (uint32_t)(16384 >> 4) << 16;  // V: leading offset of the next 64 dimensions
+                constexpr uint32_t step = L::kTile >> 4;
+                auto qk = [&](int t, int stage) {
+                    const uint32_t kb = ring_lo + stage * step, qb = q_lo + t * step;
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t o = (kk >> 2) * 16384 + (kk & 3) * 32;
-                        pk_mma_ss(tmem + t * 128, pk_desc(qb + o, 16), pk_desc(kb + o, 16), id_qk, kk != 0);
+                        const uint32_t o = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                        pk_mma_ss(tmem + t * 128, pk_join(qb + o, hi), pk_join(kb + o, hi), id_qk, kk != 0);
                     }
                     pk_commit(&B->s_full[t]);
                 };
-                auto pv = [&](int t, int j, int half) {
-                    const uint32_t vb = ring + ((2 * j + 1) % ST) * L::kTile;
+                auto pv = [&](int t, int stage, int half, uint32_t acc) {
+                    const uint32_t vb = (ring_lo & 0xffffu) + stage * step + mn + half * (4 * 2048 >> 4);
+                    const uint32_t pb = tmem + t * 128 + 32 * half;
 #pragma unroll
-                    for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                        pk_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * kk, pk_desc(vb + kk * 2048, 16384), id_pv,
-                                  (j | kk) != 0);
+                    for (int kk = 0; kk < 4; ++kk)
+                        pk_mma_ts(tmem + 256 + t * 128, pb + 8 * kk, pk_join(vb + kk * (2048 >> 4), hi), id_pv, acc | kk);
                 };
-                if (!mbar_wait_bounded(&B->q_full, 0, a.err, 53)) ok = false;
-                wait_kv(0);
+                // A wait costs 150 to 200 cycles even when its barrier is done (it queues behind
+                // the softmax warps' exponentials), so the waits for K and V come while the first
+                // tile's softmax still runs, and the commits that nobody waits for come last.
+                int stage = 0;
+                uint32_t phase = 0;
+                auto next = [&]() {
+                    if (++stage == ST) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                };
+                ok = pk_wait(&B->q_full, 0, a.err, 53) && pk_wait(&B->kv_full[0], 0, a.err, 52);
                 if (ok) {
                     pk_fence_after();
                     if (n0 > 0) qk(0, 0);
                     if (n1 > 0) qk(1, 0);
                     pk_commit(&B->kv_empty[0]);
                 }
+                next();
+#pragma unroll 1
                 for (int j = 0; j < nb && ok; ++j) {
-                    wait_kv(2 * j + 1);
-                    if (j >= part && ok && !mbar_wait_bounded(&B->v_clean[(j - part) & 3], ((j - part) >> 2) & 1, a.err, 54))
-                        ok = false;
-                    if (j + 1 < nb) wait_kv(2 * j + 2);
-                    for (int t = 0; t < 2 && ok; ++t) {
+                    const int vs = stage;
+                    ok = pk_wait(&B->kv_full[vs], phase, a.err, 52);
+                    if (j >= part) ok = ok && pk_wait(&B->v_clean[(j - part) & 3], ((j - part) >> 2) & 1, a.err, 54);
+                    next();
+                    const int ks = stage;
+                    if (j + 1 < nb) ok = ok && pk_wait(&B->kv_full[ks], phase, a.err, 52);
+                    next();
+#pragma unroll 1
+                    for (int t = 0; t < 2; ++t) {
                         const int nt = t ? n1 : n0;
                         if (j < nt) {
-                            if (!mbar_wait_bounded(&B->p_half[t], j & 1, a.err, 55)) {
-                                ok = false;
-                                break;
-                            }
+                            ok = ok && pk_wait(&B->p_half[t], j & 1, a.err, 55);
+                            if (!ok) break;
                             pk_fence_after();
-                            pv(t, j, 0);
-                            if (!mbar_wait_bounded(&B->p_full[t], j & 1, a.err, 60)) {
-                                ok = false;
-                                break;
-                            }
+                            pv(t, vs, 0, j);
+                            ok = pk_wait(&B->p_full[t], j & 1, a.err, 60);
+                            if (!ok) break;
                             pk_fence_after();
-                            pv(t, j, 1);
+                            pv(t, vs, 1, 1);
                             if (j + 1 == nt) pk_commit(&B->o_full[t]);
                         }
-                        if (t == 1) pk_commit(&B->kv_empty[(2 * j + 1) % ST]);
-                        if (j + 1 < nt) qk(t, j + 1);
+                        if (j + 1 < nt) qk(t, ks);
                     }
-                    if (j + 1 < nb && ok) pk_commit(&B->kv_empty[(2 * j + 2) % ST]);
+                    if (ok) {
+                        pk_commit(&B->kv_empty[vs]);
+                        if (j + 1 < nb) pk_commit(&B->kv_empty[ks]);
+                    }
                 }
             }
         } else {
@@ -474,7 +510,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             const int ct = tid - 320;  // 0..63
             for (int j = part; j < nb && ok; ++j) {
                 const int s = (2 * j + 1) % ST, c = j - part;
-                if (!mbar_wait_bounded(&B->v_raw[c & 3], (c >> 2) & 1, a.err, 56)) {
+                if (!pk_wait(&B->v_raw[c & 3], (c >> 2) & 1, a.err, 56)) {
                     ok = false;
                     break;
                 }
@@ -531,7 +567,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to
             for (int j = 0; j < nt; ++j) {
                 // (the warp leaves as one: what follows is warp-wide)
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&B->s_full[t], j & 1, a.err, 57))) {
+                if (!__all_sync(0xffffffffu, pk_wait(&B->s_full[t], j & 1, a.err, 57))) {
                     ok = false;
                     break;
                 }
@@ -546,9 +582,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     for (int i = 0; i < 128; ++i)
                         if (i > seen) sv[i] = 0xff800000u;
                 }
-                // exponentials of keys 64 c .. 64 c + 63, their sum and P
+                // exponentials of keys 64 c .. 64 c + 63, their sum and P; FIND: the maximum of the
+                // block's 128 scores on the way (it uses another pipe than the exponentials)
                 const f32x2 scale2 = pk_pair(a.scale_log2, a.scale_log2);
-                auto half = [&](int c, float m, f32x2(&sum)[2], uint32_t(&pv)[32]) {
+                float mx[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
+                auto half = [&](int c, bool find, float m, f32x2(&sum)[2], uint32_t(&pv)[32]) {
                     const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
                     const f32x2 base2 = pk_pair(base, base);
                     sum[0] = sum[1] = 0;
@@ -558,26 +598,20 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         float2 u = pk_unpair(x);
                         u.x = pk_ex2(u.x);
                         u.y = pk_ex2(u.y);
+                        if (find) {
+                            float &p = mx[(2 * i) & 3], &r = mx[(2 * i + 1) & 3];
+                            p = pk_max3(p, __uint_as_float(sv[4 * i]), __uint_as_float(sv[4 * i + 1]));
+                            r = pk_max3(r, __uint_as_float(sv[4 * i + 2]), __uint_as_float(sv[4 * i + 3]));
+                        }
                         sum[i & 1] = pk_add2(sum[i & 1], pk_pair(u.x, u.y));
                         pv[i] = PkType<T>::pack(u.x, u.y);
                     }
                 };
                 // The first half is computed with the maximum so far while this block's is
-                // found (the exponentials and the maximum use different pipes), and again
-                // in the rare case that the maximum moves.
+                // found, and again in the rare case that the maximum moves.
                 f32x2 sum[2];
                 uint32_t pv[32];
-                half(0, m, sum, pv);
-                float mx[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
-#pragma unroll
-                for (int i = 4; i < 124; i += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mx[e] = pk_max3(mx[e], __uint_as_float(sv[i + e]), __uint_as_float(sv[i + 4 + e]));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = pk_max3(mx[e], __uint_as_float(sv[124 + e]), mx[e]);
+                half(0, true, m, sum, pv);
                 const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 if (mb != mb) l = mb;  // a key that this row sees scores NaN: so does the row
                 const bool move = (mb - m) * a.scale_log2 > 8.f || (m == -INFINITY && mb > m);
@@ -597,12 +631,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                             pk_st(o_t + 32 * c, ov);
                         }
                     }
-                    half(0, m, sum, pv);
+                    half(0, false, m, sum, pv);
                 }
                 // P goes to the tensor cores in two halves, the first while the second is computed
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    if (c) half(1, m, sum, pv);
+                    if (c) half(1, false, m, sum, pv);
                     const float2 u = pk_unpair(pk_add2(sum[0], sum[1]));
                     l += u.x + u.y;
                     pk_st(s_t + 32 * c, pv);
@@ -612,10 +646,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 }
             }
             // ---- epilogue
-            if (nt > 0 && ok && !__all_sync(0xffffffffu, mbar_wait_bounded(&B->o_full[t], 0, a.err, 58))) ok = false;
+            if (nt > 0 && ok && !__all_sync(0xffffffffu, pk_wait(&B->o_full[t], 0, a.err, 58))) ok = false;
             pk_fence_after();
             // what the clearing warps noted of this tile's blocks
-            if (nt > part && ok) mbar_wait_bounded(&B->v_clean[(nt - 1 - part) & 3], ((nt - 1 - part) >> 2) & 1, a.err, 59);
+            if (nt > part && ok) pk_wait(&B->v_clean[(nt - 1 - part) & 3], ((nt - 1 - part) >> 2) & 1, a.err, 59);
             const int h = chunk * a.GT + row % a.GT;
             const bool mine = row < PT * a.GT && jq < ql && h < a.G && ok;
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
