@@ -170,6 +170,23 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Store a) {
 }
 
 // ------------------------------------------------------------------ attention
+// Per row and K/V head, G query heads share the keys, 8 NG of them per CTA:
+//   S^T[keys x heads] = K Q^T    m16n8k16, keys in M, 8 heads in N
+//   P   = exp2(c (S s_k - m))    m moves only when it is 2^8 behind (as in the prompt kernel)
+//   O^T[dims x heads] += s_v (V^T P)
+// The cache is read once, straight into the registers that hold the A operands:
+// the contraction of Q K^T runs over dims in the order in which 16-byte pieces of
+// a K row fall to the four lanes of a row group, and V^T is formed from the bytes of four
+// keys by permutes, so no shared memory and no barrier stands between HBM and
+// the tensor cores.  e4m3 converts to fp16 exactly; bf16 queries are brought to
+// fp16 by a power of two per head (their largest value to [2^14, 2^15)).
+// A warp takes 32 keys at a time and keeps the next 32 keys' K and V in flight.
+// A cluster of CTAs shares a (row, K/V head) and joins its parts (m, l, O) through
+// distributed shared memory; contexts that are long for the number of pairs are
+// split over several clusters, whose parts go through the caller's workspace.
+constexpr int kAtWarps = 4;
+constexpr int kAtKeys = 32;  // keys per warp and step
+
 struct Kv8Attn {
     void *out;
     long out_rs;
@@ -181,74 +198,450 @@ struct Kv8Attn {
     const int *table;
     int n_seqs, max_pages;
     const int *seq, *pos;
-    int heads, kv_heads;
-    float scale;
+    int heads, kv_heads, G, chunks;  // chunks of 8 NG heads per K/V head
+    float scale_log2;
+    int vec;       // q rows are 8-byte aligned
+    int cluster;   // CTAs that share a (row, K/V head, split)
+    int splits;
+    float *part;   // [rows][heads][splits][D + 2] when splits > 1: O, m, l
 };
 
-__device__ __forceinline__ float e4m3_to_float(uint8_t b) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
+__device__ __forceinline__ uint4 ldg_stream16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+// two e4m3 codes (low 16 bits of w) -> half2, exact
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    return (uint32_t)r.x | (uint32_t)r.y << 16;
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
+    uint32_t a = smem_u32(p), r;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+    return v;
 }
 
-// One CTA per (row, query head), 128 threads: a thread scores one key of each
-// block of 128, then owns one dimension of the output.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv8_attn_kernel(Kv8Attn a) {
-    __shared__ float s_q[D], s_p[128], s_w[4];
-    __shared__ int s_page[2];
-    const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const int kh = h / (a.heads / a.kv_heads);
+template <typename T> struct Kv8Q {
+    static constexpr bool rescale = false;
+};
+template <> struct Kv8Q<__nv_bfloat16> {
+    static constexpr bool rescale = true;
+};
+
+// grid: (cluster * chunks * kv_heads, rows, splits)
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a) {
+    constexpr int HB = 8 * NG;       // heads per CTA
+    constexpr int KC = D / 64;       // 16-byte pieces of a K row per lane
+    constexpr int MT = D / 16;       // 16-dim tiles of O
+    constexpr int VW = D / 32;       // 32-bit words of a V row per lane
+    __shared__ float s_o[kAtWarps][HB][D];
+    __shared__ float s_m[kAtWarps][HB], s_l[kAtWarps][HB];
+    __shared__ float s_co[HB][D], s_cm[HB], s_cl[HB];  // this CTA's part, read by the cluster
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int rank = blockIdx.x % a.cluster, hc = blockIdx.x / a.cluster;
+    const int kvh = hc / a.chunks, h0 = (hc % a.chunks) * HB;  // first head, within the group
+    const int row = blockIdx.y;
     pdl_wait();
     pdl_trigger();
     const int seq = a.seq[row];
-    const long len = seq >= 0 && seq < a.n_seqs
-                         ? min((long)a.pos[row] + 1, (long)a.max_pages * kKv8Page) : 0;
-    if (tid < D) s_q[tid] = to_float(reinterpret_cast<const T *>(a.q)[row * a.q_rs + h * D + tid]) * a.scale;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (long k0 = 0; k0 < len; k0 += 128) {
-        __syncthreads();
-        if (tid < 2) {
-            const long p = k0 / kKv8Page + tid;
-            const int page = p < a.max_pages ? a.table[(long)seq * a.max_pages + p] : -1;
-            s_page[tid] = page < a.n_pages ? page : -1;
+    const long len = seq >= 0 && seq < a.n_seqs ? min((long)a.pos[row] + 1, (long)a.max_pages * kKv8Page) : 0;
+    const int *table = a.table + (long)(len > 0 ? seq : 0) * a.max_pages;
+    const int units = len > 0 ? (int)((len + kAtKeys - 1) / kAtKeys) : 0;
+    const int gw = ((int)blockIdx.z * a.cluster + rank) * kAtWarps + warp, TW = a.splits * a.cluster * kAtWarps;
+    const size_t head_bytes = (size_t)kKv8Page * D, page_bytes = head_bytes * a.kv_heads;
+
+    uint4 kr[4][KC];   // K: rows g, g + 8, g + 16, g + 24 of the step's keys
+    uint32_t vr[8][VW];  // V: keys 2t, 2t + 1, 2t + 8, 2t + 9 of both 16-key tiles; dims VW * 4 * g ..
+    int page = -1, next_page = -1;  // of the step in registers, of the one after
+    float ks = 0.f, vs = 0.f;
+    auto page_of = [&](int u) -> int {
+        if (u >= units) return -1;
+        const int p = table[u >> 1];
+        return p >= 0 && p < a.n_pages ? p : -1;
+    };
+    auto load_k = [&](int u, int p) {
+        if (p < 0) return;
+        const uint8_t *b = a.kpool + p * page_bytes + kvh * head_bytes + (u & 1) * (kAtKeys * D) + g * D + t * 16;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) kr[r][c] = ldg_stream16(b + r * 8 * D + c * 64);
+    };
+    auto load_v = [&](int u, int p) {
+        if (p < 0) return;
+        const uint8_t *b = a.vpool + p * page_bytes + kvh * head_bytes + (u & 1) * (kAtKeys * D) + 2 * t * D + g * (VW * 4);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const uint8_t *x = b + ((r >> 2) * 16 + (r & 1) + ((r >> 1) & 1) * 8) * D;
+            if (VW == 4) {
+                const uint4 v = ldg_stream16(x);
+                vr[r][0] = v.x, vr[r][1] = v.y, vr[r][VW > 2 ? 2 : 0] = v.z, vr[r][VW > 2 ? 3 : 0] = v.w;
+            } else {
+                const uint2 v = ldg_stream8(x);
+                vr[r][0] = v.x, vr[r][1] = v.y;
+            }
         }
-        __syncthreads();
-        float s = -INFINITY;
-        const int page = s_page[tid / kKv8Page];
-        if (k0 + tid < len && page >= 0) {
-            const long ps = (long)page * a.kv_heads + kh;
-            const uint8_t *k = a.kpool + (ps * kKv8Page + tid % kKv8Page) * D;
-            float dot = 0.f;
-            for (int d = 0; d < D; ++d) dot += s_q[d] * e4m3_to_float(k[d]);
-            s = dot * a.kscale[ps];
+    };
+    page = page_of(gw);
+    next_page = page_of(gw + TW);
+    load_k(gw, page);
+    load_v(gw, page);
+    if (page >= 0) {
+        ks = a.kscale[(long)page * a.kv_heads + kvh];
+        vs = a.vscale[(long)page * a.kv_heads + kvh];
+    }
+
+    // ---- queries: B operand, lane (g, t) holds head g, dims 64 c + 16 t + 4 k .. + 3
+    uint32_t qb[NG][KC * 4][2];
+    float c0[NG], c1[NG];  // of heads 2t, 2t + 1: what a product of codes counts, in log2
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        const int h = h0 + n * 8 + g;
+        const T *q = reinterpret_cast<const T *>(a.q) + (long)row * a.q_rs + (long)(kvh * a.G + h) * D + 16 * t;
+        T x[KC * 4][4];
+#pragma unroll
+        for (int k = 0; k < KC * 4; ++k) {
+            const T *src = q + (k >> 2) * 64 + (k & 3) * 4;
+            uint2 u = make_uint2(0, 0);
+            if (h < a.G) {
+                if (a.vec) {
+                    u = *reinterpret_cast<const uint2 *>(src);
+                } else {
+                    const unsigned short *e = reinterpret_cast<const unsigned short *>(src);
+                    u.x = e[0] | (uint32_t)e[1] << 16;
+                    u.y = e[2] | (uint32_t)e[3] << 16;
+                }
+            }
+            *reinterpret_cast<uint2 *>(x[k]) = u;
         }
-        float bm = warp_max(s);
-        if (lane == 0) s_w[wid] = bm;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(s_w[0], s_w[1]), fmaxf(s_w[2], s_w[3])));
-        const float p = s == -INFINITY ? 0.f : expf(s - mn);
-        s_p[tid] = p;
-        __syncthreads();
-        const float ps_ = warp_sum(p);
-        if (lane == 0) s_w[wid] = ps_;
-        __syncthreads();
-        const float c = mn == -INFINITY ? 1.f : expf(m - mn);
-        l = l * c + (s_w[0] + s_w[1] + s_w[2] + s_w[3]);
-        o *= c;
-        m = mn;
-        if (tid < D) {
-            for (int b = 0; b < 2; ++b) {
-                if (s_page[b] < 0) continue;
-                const long ps = (long)s_page[b] * a.kv_heads + kh;
-                const uint8_t *v = a.vpool + ps * kKv8Page * D + tid;
-                const int n = (int)min(len - k0 - b * kKv8Page, (long)kKv8Page);
-                float acc = 0.f;
-                for (int j = 0; j < n; ++j) acc += s_p[b * kKv8Page + j] * e4m3_to_float(v[j * D]);
-                o += acc * a.vscale[ps];
+        float f = 1.f;
+        if (Kv8Q<T>::rescale) {
+            float m = 0.f;
+#pragma unroll
+            for (int k = 0; k < KC * 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(to_float(x[k][e])));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const int e = max((int)(__float_as_uint(m) >> 23) - 127, -100);
+            f = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+#pragma unroll
+            for (int k = 0; k < KC * 4; ++k)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const __half2 v = __floats2half2_rn(to_float(x[k][2 * p]) * f, to_float(x[k][2 * p + 1]) * f);
+                    qb[n][k][p] = *reinterpret_cast<const uint32_t *>(&v);
+                }
+            f = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+        } else {
+#pragma unroll
+            for (int k = 0; k < KC * 4; ++k)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) qb[n][k][p] = reinterpret_cast<const uint32_t *>(x[k])[p];
+        }
+        c0[n] = __shfl_sync(0xffffffffu, f, 8 * t) * a.scale_log2;
+        c1[n] = __shfl_sync(0xffffffffu, f, 8 * t + 4) * a.scale_log2;
+    }
+
+    float o[NG][MT][4], m0[NG], m1[NG], l0[NG], l1[NG];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        m0[n] = m1[n] = -INFINITY;
+        l0[n] = l1[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+    }
+    for (int u = gw; u < units; u += TW) {
+        const int cur = page;
+        const float cks = ks, cvs = vs;
+        page = next_page;
+        next_page = page_of(u + 2 * TW);
+        if (page >= 0) {
+            ks = a.kscale[(long)page * a.kv_heads + kvh];
+            vs = a.vscale[(long)page * a.kv_heads + kvh];
+        }
+        uint32_t pb[NG][2][2];
+        if (cur >= 0) {
+            // ---- scores of 32 keys
+            float s[NG][2][4];
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][i][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k = 0; k < KC * 4; ++k) {
+                    const uint32_t w0 = reinterpret_cast<const uint32_t *>(&kr[2 * i][k >> 2])[k & 3];
+                    const uint32_t w1 = reinterpret_cast<const uint32_t *>(&kr[2 * i + 1][k >> 2])[k & 3];
+                    const uint32_t a0 = e4m3x2_to_h2(w0), a2 = e4m3x2_to_h2(w0 >> 16);
+                    const uint32_t a1 = e4m3x2_to_h2(w1), a3 = e4m3x2_to_h2(w1 >> 16);
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) mma_f16(s[n][i], a0, a1, a2, a3, qb[n][k][0], qb[n][k][1]);
+                }
+            load_k(u + TW, page);
+            // ---- softmax: lane holds heads 2t (e = 0, 2) and 2t + 1 (1, 3), keys g (e < 2) and g + 8
+            const int left = (int)min(len - (long)u * kAtKeys, (long)kAtKeys);  // keys that the row sees
+            bool move = false;
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                const float f0 = c0[n] * cks, f1 = c1[n] * cks;
+                float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool seen = i * 16 + (e >> 1) * 8 + g < left;
+                        s[n][i][e] = seen ? s[n][i][e] * ((e & 1) ? f1 : f0) : -INFINITY;
+                        if (e & 1)
+                            x1 = fmaxf(x1, s[n][i][e]);
+                        else
+                            x0 = fmaxf(x0, s[n][i][e]);
+                    }
+                move |= x0 - m0[n] > 8.f || x1 - m1[n] > 8.f;
+                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+                        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                    }
+                    const float y0 = fmaxf(m0[n], x0), y1 = fmaxf(m1[n], x1);
+                    const float r0 = m0[n] == y0 || m0[n] == -INFINITY ? 1.f : ex2(m0[n] - y0);
+                    const float r1 = m1[n] == y1 || m1[n] == -INFINITY ? 1.f : ex2(m1[n] - y1);
+                    m0[n] = y0;
+                    m1[n] = y1;
+                    l0[n] *= r0;
+                    l1[n] *= r1;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        o[n][i][0] *= r0;
+                        o[n][i][1] *= r1;
+                        o[n][i][2] *= r0;
+                        o[n][i][3] *= r1;
+                    }
+                }
+                const float b0 = m0[n] == -INFINITY ? 0.f : m0[n], b1 = m1[n] == -INFINITY ? 0.f : m1[n];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[n][i][e] = ex2(s[n][i][e] - ((e & 1) ? b1 : b0));
+                        if (e & 1)
+                            l1[n] += s[n][i][e];
+                        else
+                            l0[n] += s[n][i][e];
+                    }
+                    // P^T as the B operand: (key, heads) pairs -> (head, keys) pairs
+                    const __half2 lo = __floats2half2_rn(s[n][i][0], s[n][i][1]);
+                    const __half2 hi = __floats2half2_rn(s[n][i][2], s[n][i][3]);
+                    pb[n][i][0] = movmatrix_t(*reinterpret_cast<const uint32_t *>(&lo));
+                    pb[n][i][1] = movmatrix_t(*reinterpret_cast<const uint32_t *>(&hi));
+                }
+            }
+            if (left < kAtKeys) {  // codes behind the end may be anything, NaN included
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if ((r >> 2) * 16 + 2 * t + (r & 1) + ((r >> 1) & 1) * 8 >= left)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vr[r][w] = 0;
+            }
+            // ---- O^T += s_v V^T P: dims VW 4 g + 4 w + 2 j (row g) and + 1 (row g + 8) in tile 2 w + j
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                float acc[NG][2][4];
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t x[2][2];  // [keys 2t, 2t + 1 | 2t + 8, 2t + 9][dims 0, 1 | 2, 3], key pairs per dim
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        x[p][0] = __byte_perm(vr[4 * i + 2 * p][w], vr[4 * i + 2 * p + 1][w], 0x5140);
+                        x[p][1] = __byte_perm(vr[4 * i + 2 * p][w], vr[4 * i + 2 * p + 1][w], 0x7362);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t a0 = e4m3x2_to_h2(x[0][j]), a1 = e4m3x2_to_h2(x[0][j] >> 16);
+                        const uint32_t a2 = e4m3x2_to_h2(x[1][j]), a3 = e4m3x2_to_h2(x[1][j] >> 16);
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) mma_f16(acc[n][j], a0, a1, a2, a3, pb[n][i][0], pb[n][i][1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][2 * w + j][e] = fmaf(acc[n][j][e], cvs, o[n][2 * w + j][e]);
+            }
+        } else {
+            load_k(u + TW, page);
+        }
+        load_v(u + TW, page);
+    }
+
+    // ---- join the warps, then the cluster's CTAs, then (another launch) the splits
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+            l0[n] += __shfl_xor_sync(0xffffffffu, l0[n], d);
+            l1[n] += __shfl_xor_sync(0xffffffffu, l1[n], d);
+        }
+        const int h = n * 8 + 2 * t;
+        if (g == 0) {
+            s_m[warp][h] = m0[n];
+            s_m[warp][h + 1] = m1[n];
+            s_l[warp][h] = l0[n];
+            s_l[warp][h + 1] = l1[n];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int d = VW * 4 * g + 2 * i;
+            *reinterpret_cast<float2 *>(&s_o[warp][h][d]) = make_float2(o[n][i][0], o[n][i][2]);
+            *reinterpret_cast<float2 *>(&s_o[warp][h + 1][d]) = make_float2(o[n][i][1], o[n][i][3]);
+        }
+    }
+    __syncthreads();
+    const int nh = min(HB, a.G - h0);
+    auto put = [&](int h, int d, float m, float l, float v) {  // the joined part of a cluster
+        const long at = (long)row * a.heads + kvh * a.G + h0 + h;
+        if (a.splits == 1) {
+            reinterpret_cast<T *>(a.out)[(long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d] =
+                from_float<T>(l > 0.f || l != l ? v / l : 0.f);
+        } else {
+            float *p = a.part + (at * a.splits + blockIdx.z) * (D + 2);
+            p[d] = v;
+            if (d == 0) {
+                p[D] = m;
+                p[D + 1] = l;
+            }
+        }
+    };
+    for (int x = tid; x < nh * D; x += kAtWarps * 32) {
+        const int h = x / D, d = x % D;
+        float m = s_m[0][h];
+#pragma unroll
+        for (int w = 1; w < kAtWarps; ++w) m = fmaxf(m, s_m[w][h]);
+        float l = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAtWarps; ++w) {
+            const float f = s_m[w][h] == -INFINITY ? (s_l[w][h] != s_l[w][h] ? 1.f : 0.f) : ex2(s_m[w][h] - m);
+            l += s_l[w][h] * f;
+            v += s_o[w][h][d] * f;
+        }
+        if (a.cluster == 1) {
+            put(h, d, m, l, v);
+        } else {
+            s_co[h][d] = v;
+            if (d == 0) {
+                s_cm[h] = m;
+                s_cl[h] = l;
             }
         }
     }
-    if (tid < D)
-        reinterpret_cast<T *>(a.out)[row * a.out_rs + h * D + tid] = from_float<T>(l > 0.f || l != l ? o / l : 0.f);
+    if (a.cluster > 1) {
+        cluster_sync_all();
+        const int share = (nh * D + a.cluster - 1) / a.cluster;
+        const int x1 = min(nh * D, (rank + 1) * share);
+        for (int x = rank * share + tid; x < x1; x += kAtWarps * 32) {
+            const int h = x / D, d = x % D;
+            float m = -INFINITY;
+            for (int c = 0; c < a.cluster; ++c) m = fmaxf(m, ld_cluster(&s_cm[h], c));
+            float l = 0.f, v = 0.f;
+            for (int c = 0; c < a.cluster; ++c) {
+                const float mc = ld_cluster(&s_cm[h], c), lc = ld_cluster(&s_cl[h], c);
+                const float f = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - m);
+                l += lc * f;
+                v += ld_cluster(&s_co[h][d], c) * f;
+            }
+            put(h, d, m, l, v);
+        }
+        cluster_sync_all();  // no CTA leaves while its part is read
+    }
+}
+
+// out = sum over splits of O 2^(m - max), over the sum of l 2^(m - max): one CTA per (head, row)
+template <typename T, int D>
+__global__ void __launch_bounds__(D * 4) kv8_join_kernel(T *__restrict__ out, long out_rs,
+                                                         const float *__restrict__ part, int heads, int splits) {
+    __shared__ float s_v[4][D], s_l[4][D];
+    const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x % D, q = threadIdx.x / D;
+    pdl_wait();
+    pdl_trigger();
+    const float *p = part + ((long)row * heads + h) * splits * (D + 2);
+    float m = -INFINITY;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, p[(long)s * (D + 2) + D]);
+    float l = 0.f, v = 0.f;
+    for (int s = q; s < splits; s += 4) {
+        const float *x = p + (long)s * (D + 2);
+        const float mc = x[D], lc = x[D + 1];
+        const float f = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - m);
+        l += lc * f;
+        v += x[d] * f;
+    }
+    s_v[q][d] = v;
+    s_l[q][d] = l;
+    __syncthreads();
+    if (q == 0) {
+        v = (s_v[0][d] + s_v[1][d]) + (s_v[2][d] + s_v[3][d]);
+        l = (s_l[0][d] + s_l[1][d]) + (s_l[2][d] + s_l[3][d]);
+        out[row * out_rs + (long)h * D + d] = from_float<T>(l > 0.f || l != l ? v / l : 0.f);
+    }
+}
+
+// How a call's context is shared out.
+struct Kv8Split {
+    int ng, chunks, cluster, splits;
+};
+Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int sms) {
+    Kv8Split s;
+    const int G = heads / kv_heads;
+    s.ng = G <= 8 ? 1 : 2;
+    s.chunks = (G + 8 * s.ng - 1) / (8 * s.ng);
+    const long pairs = (long)rows * kv_heads * s.chunks;
+    const int units = max_len > 0 ? (max_len - 1) / kAtKeys + 1 : 1;
+    const long ctas = 3l * sms;                                    // that run at a time
+    const int useful = (units + kAtWarps - 1) / kAtWarps;          // CTAs with a step for every warp
+    long want = (ctas + pairs - 1) / pairs;                        // fill the machine
+    const int tail = (units + 16 * kAtWarps - 1) / (16 * kAtWarps);  // at most 16 steps per warp
+    if (want < tail) want = tail;
+    if (want > useful) want = useful;
+    s.cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
+    s.splits = want > 8 ? (int)(want / 8) : 1;
+    return s;
 }
 
 template <typename T, int D> cudaError_t launch_store(const Kv8Store &a, int units, cudaStream_t s) {
@@ -267,17 +660,42 @@ template <typename T, int D> cudaError_t launch_store(const Kv8Store &a, int uni
                : cudaLaunchKernelEx(&cfg, kv8_store_kernel<T, D, false>, a);
 }
 
-template <typename T, int D> cudaError_t launch_attn(const Kv8Attn &a, int rows, cudaStream_t s) {
+template <typename T, int D, int NG>
+cudaError_t launch_attn_ng(const Kv8Attn &a, int rows, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.cluster * a.chunks * a.kv_heads, rows, a.splits);
+    cfg.blockDim = dim3(kAtWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_rt.pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D, NG>, a);
+}
+
+template <typename T, int D> cudaError_t launch_attn(const Kv8Attn &a, int ng, int rows, cudaStream_t s) {
+    cudaError_t e = ng == 1 ? launch_attn_ng<T, D, 1>(a, rows, s) : launch_attn_ng<T, D, 2>(a, rows, s);
+    if (e != cudaSuccess || a.splits == 1) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.heads, rows);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(4 * D);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = g_rt.pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D>, a);
+    return cudaLaunchKernelEx(&cfg, kv8_join_kernel<T, D>, (T *)a.out, a.out_rs, (const float *)a.part, a.heads,
+                              a.splits);
+}
+
+long long kv8_ws_bytes(int rows, int heads, int head_dim, int splits) {
+    return splits > 1 ? 4ll * rows * heads * splits * (head_dim + 2) : 0;
 }
 
 }  // namespace
@@ -319,8 +737,9 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
 }
 
 long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim) {
-    (void)rows, (void)max_len, (void)n_heads, (void)kv_heads, (void)head_dim;
-    return 0;
+    if (rows < 1 || max_len < 1 || kv_heads < 1 || n_heads < 1 || n_heads % kv_heads || head_dim < 1) return 0;
+    const int sms = g_rt.num_sms > 0 ? g_rt.num_sms : 148;
+    return kv8_ws_bytes(rows, n_heads, head_dim, kv8_split(rows, max_len, n_heads, kv_heads, sms).splits);
 }
 
 int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
@@ -341,16 +760,41 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
         return fail("wk_kv8_attention: pools must be 16-byte aligned");
     if (g_rt.device < 0) return fail("wk_kv8_attention: cuda_init() has not been called");
     DeviceGuard guard;
-    Kv8Attn a{out, out_rs, q, q_rs, (const uint8_t *)kpool, (const uint8_t *)vpool, kscale, vscale, n_pages,
-              block_table, n_seqs, max_pages, seq, pos, n_heads, kv_heads, 1.0f / sqrtf((float)head_dim)};
+    Kv8Split sp = kv8_split(rows, max_len, n_heads, kv_heads, g_rt.num_sms);
+    if (!ws || ((uintptr_t)ws % 16)) ws_bytes = 0;
+    while (sp.splits > 1 && kv8_ws_bytes(rows, n_heads, head_dim, sp.splits) > ws_bytes) --sp.splits;
+    Kv8Attn a;
+    a.out = out;
+    a.out_rs = out_rs;
+    a.q = q;
+    a.q_rs = q_rs;
+    a.kpool = (const uint8_t *)kpool;
+    a.vpool = (const uint8_t *)vpool;
+    a.kscale = kscale;
+    a.vscale = vscale;
+    a.n_pages = n_pages;
+    a.table = block_table;
+    a.n_seqs = n_seqs;
+    a.max_pages = max_pages;
+    a.seq = seq;
+    a.pos = pos;
+    a.heads = n_heads;
+    a.kv_heads = kv_heads;
+    a.G = n_heads / kv_heads;
+    a.chunks = sp.chunks;
+    a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
+    a.vec = ((uintptr_t)q % 8) == 0 && q_rs % 4 == 0;
+    a.cluster = sp.cluster;
+    a.splits = sp.splits;
+    a.part = (float *)ws;
     cudaStream_t s = stream();
     cudaError_t e;
     if (dtype == kF16)
-        e = head_dim == 64 ? launch_attn<__half, 64>(a, rows, s) : launch_attn<__half, 128>(a, rows, s);
+        e = head_dim == 64 ? launch_attn<__half, 64>(a, sp.ng, rows, s) : launch_attn<__half, 128>(a, sp.ng, rows, s);
     else
-        e = head_dim == 64 ? launch_attn<__nv_bfloat16, 64>(a, rows, s) : launch_attn<__nv_bfloat16, 128>(a, rows, s);
+        e = head_dim == 64 ? launch_attn<__nv_bfloat16, 64>(a, sp.ng, rows, s)
+                           : launch_attn<__nv_bfloat16, 128>(a, sp.ng, rows, s);
     if (e != cudaSuccess) return fail("wk_kv8_attention: %s", cudaGetErrorString(e));
-    (void)ws;
     return 0;
 }
 
