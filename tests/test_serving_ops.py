@@ -143,6 +143,7 @@ def test_store_refusals(change, words):
     (dict(ws_bytes=-1), "bad sizes"), (dict(heads=3), "3 heads over 2"), (dict(heads=0), "heads"),
     (dict(hd=32), "head_dim 32"), (dict(dt=wk.Q8_0), "dtype 8"), (dict(q=None), "null"), (dict(pos=None), "null"),
     (dict(q_rs=255), "stride"), (dict(out_rs=1), "stride"), (dict(vpool=FAKE + 4), "aligned"),
+    (dict(ws=FAKE + 4, ws_bytes=99), "workspace"),
 ])
 def test_decode_refusals(change, words):
     a = dict(out=FAKE, out_rs=256, q=FAKE, q_rs=256, kpool=FAKE, vpool=FAKE, kscale=FAKE, vscale=FAKE, n_pages=4,

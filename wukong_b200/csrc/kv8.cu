@@ -181,10 +181,17 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Store a) {
 // the tensor cores.  e4m3 converts to fp16 exactly; bf16 queries are brought to
 // fp16 by a power of two per head (their largest value to [2^14, 2^15)).
 // A warp takes 32 keys at a time and keeps the next 32 keys' K and V in flight.
-// A cluster of CTAs shares a (row, K/V head) and joins its parts (m, l, O) through
-// distributed shared memory; contexts that are long for the number of pairs are
-// split over several clusters, whose parts go through the caller's workspace.
+// The context is shared out in one of two ways:
+//   clusters  a cluster of CTAs takes one (row, K/V head) and joins its parts
+//             (m, l, O) through distributed shared memory: one launch
+//   even      the steps of all rows and K/V heads, one after the other, are cut into as
+//             many equal runs as CTAs fit on the GPU; a run that ends inside a
+//             (row, K/V head) leaves its part in the caller's workspace, and a second
+//             launch joins those
 constexpr int kAtWarps = 4;
+#ifndef WK_EVENMIN
+#define WK_EVENMIN 8
+#endif
 constexpr int kAtKeys = 32;  // keys per warp and step
 
 struct Kv8Attn {
@@ -201,10 +208,25 @@ struct Kv8Attn {
     int heads, kv_heads, G, chunks;  // chunks of 8 NG heads per K/V head
     float scale_log2;
     int vec;       // q rows are 8-byte aligned
-    int cluster;   // CTAs that share a (row, K/V head, split)
-    int splits;
-    float *part;   // [rows][heads][splits][D + 2] when splits > 1: O, m, l
+    int rows;
+    int cluster;   // CTAs that share a (row, K/V head)
+    int ctas;      // even shares: CTAs of the launch
+    int *prefix;   // even shares: [rows + 1] cost of the rows before each, per head group (written by CTA 0)
+    float *part;   // even shares: [ctas][2][8 NG][D + 2]: O, m, l of a run's part of a head group
 };
+
+// Even shares: a (row, head group) of n steps costs n + kSegCost, the latencies of
+// its start and its end (lengths, table, first K and V, queries, the join of the
+// warps) being worth kSegCost steps; one without keys costs nothing.  The sum
+// `total` of the costs is cut into runs, run c being [c total / runs, (c + 1) total / runs).
+#ifndef WK_SEGCOST
+#define WK_SEGCOST 8
+#endif
+constexpr int kSegCost = WK_SEGCOST;
+__device__ __forceinline__ long long kv8_runs(long long total, int ctas) {
+    const long long most = (total + kSegCost + 7) / (kSegCost + 8);
+    return most < ctas ? (most > 0 ? most : 1) : ctas;
+}
 
 __device__ __forceinline__ uint4 ldg_stream16(const void *p) {
     uint4 v;
@@ -218,10 +240,11 @@ __device__ __forceinline__ uint2 ldg_stream8(const void *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
     return v;
 }
-// two e4m3 codes (low 16 bits of w) -> half2, exact
-__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    return (uint32_t)r.x | (uint32_t)r.y << 16;
+// four e4m3 codes -> two half2, exact
+__device__ __forceinline__ void e4m3x4_to_h2x2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
 }
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
     uint32_t r;
@@ -251,8 +274,8 @@ template <> struct Kv8Q<__nv_bfloat16> {
     static constexpr bool rescale = true;
 };
 
-// grid: (cluster * chunks * kv_heads, rows, splits)
-template <typename T, int D, int NG>
+// grid: clusters (cluster * chunks * kv_heads, rows); even shares (ctas)
+template <typename T, int D, int NG, bool kEven>
 __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a) {
     constexpr int HB = 8 * NG;       // heads per CTA
     constexpr int KC = D / 64;       // 16-byte pieces of a K row per lane
@@ -260,26 +283,100 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
     constexpr int VW = D / 32;       // 32-bit words of a V row per lane
     __shared__ float s_o[kAtWarps][HB][D];
     __shared__ float s_m[kAtWarps][HB], s_l[kAtWarps][HB];
-    __shared__ float s_co[HB][D], s_cm[HB], s_cl[HB];  // this CTA's part, read by the cluster
+    __shared__ float s_co[kEven ? 1 : HB][D], s_cm[HB], s_cl[HB];  // this CTA's part, read by the cluster
+    extern __shared__ int s_prefix[];                              // even shares: [rows + 1]
+    __shared__ int s_scan[kAtWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int rank = blockIdx.x % a.cluster, hc = blockIdx.x / a.cluster;
-    const int kvh = hc / a.chunks, h0 = (hc % a.chunks) * HB;  // first head, within the group
-    const int row = blockIdx.y;
+    const size_t head_bytes = (size_t)kKv8Page * D, page_bytes = head_bytes * a.kv_heads;
+    const int HC = a.kv_heads * a.chunks;
     pdl_wait();
     pdl_trigger();
-    const int seq = a.seq[row];
-    const long len = seq >= 0 && seq < a.n_seqs ? min((long)a.pos[row] + 1, (long)a.max_pages * kKv8Page) : 0;
-    const int *table = a.table + (long)(len > 0 ? seq : 0) * a.max_pages;
-    const int units = len > 0 ? (int)((len + kAtKeys - 1) / kAtKeys) : 0;
-    const int gw = ((int)blockIdx.z * a.cluster + rank) * kAtWarps + warp, TW = a.splits * a.cluster * kAtWarps;
-    const size_t head_bytes = (size_t)kKv8Page * D, page_bytes = head_bytes * a.kv_heads;
+    auto keys_of = [&](int row) -> long {  // that the row sees
+        const int seq = a.seq[row];
+        return seq >= 0 && seq < a.n_seqs ? max(0l, min((long)a.pos[row] + 1, (long)a.max_pages * kKv8Page)) : 0;
+    };
+    int row, rank = 0, hc;
+    int u0, u1, step;         // this warp's steps of the segment: u0, u0 + step, ... below u1
+    int seg0 = 0;              // even shares: where the run stands in the head group's cost
+    long long left_cost = 0;   // even shares: what is left of this CTA's run
+    if (kEven) {
+        // cost of the rows before each
+        int base = 0;
+        for (int r0 = 0; r0 < a.rows; r0 += kAtWarps * 32) {
+            const int r = r0 + tid;
+            int n = r < a.rows ? (int)((keys_of(r) + kAtKeys - 1) / kAtKeys) : 0;
+            if (n) n += kSegCost;
+            int in = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, in, o);
+                if (lane >= o) in += v;
+            }
+            __syncthreads();
+            if (lane == 31) s_scan[warp] = in;
+            __syncthreads();
+            int before = base + in - n;
+#pragma unroll
+            for (int w = 0; w < kAtWarps; ++w) {
+                if (w < warp) before += s_scan[w];
+                base += s_scan[w];
+            }
+            if (r < a.rows) s_prefix[r] = before;
+        }
+        if (tid == 0) s_prefix[a.rows] = base;
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (int r = tid; r <= a.rows; r += kAtWarps * 32) a.prefix[r] = s_prefix[r];
+        // rows that see nothing
+        for (int r = blockIdx.x; r < a.rows; r += a.ctas)
+            if (s_prefix[r] == s_prefix[r + 1])
+                for (int x = tid; x < a.heads * D; x += kAtWarps * 32)
+                    reinterpret_cast<T *>(a.out)[(long)r * a.out_rs + x] = from_float<T>(0.f);
+        const long long total = (long long)base * HC, runs = kv8_runs(total, a.ctas);
+        if (total == 0 || blockIdx.x >= runs) return;
+        const long long b0 = blockIdx.x * total / runs;
+        left_cost = (blockIdx.x + 1) * total / runs - b0;
+        int lo = 0, hi = a.rows;  // the last row that starts at or before b0
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((long long)s_prefix[mid] * HC <= b0)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        row = lo;
+        const int n = s_prefix[row + 1] - s_prefix[row];
+        const int rem = (int)(b0 - (long long)s_prefix[row] * HC);
+        hc = rem / n;
+        seg0 = rem % n;
+    } else {
+        rank = blockIdx.x % a.cluster;
+        hc = blockIdx.x / a.cluster;
+        row = blockIdx.y;
+    }
+    for (;;) {  // segments of this CTA: parts of one (row, K/V head, chunk of heads) each
+    const int kvh = hc / a.chunks, h0 = (hc % a.chunks) * HB;  // first head, within the group
+    const long len = keys_of(row);
+    const int *table = a.table + (long)(len > 0 ? a.seq[row] : 0) * a.max_pages;
+    const int units = (int)((len + kAtKeys - 1) / kAtKeys);
+    const int cut = (int)min((long long)units + kSegCost, seg0 + left_cost);  // even shares: where the run leaves it
+    const int first = max(seg0 - kSegCost, 0);
+    if (kEven) {
+        u0 = first + warp;
+        u1 = cut - kSegCost;
+        step = kAtWarps;
+    } else {
+        u0 = rank * kAtWarps + warp;
+        u1 = units;
+        step = a.cluster * kAtWarps;
+    }
 
     uint4 kr[4][KC];   // K: rows g, g + 8, g + 16, g + 24 of the step's keys
     uint32_t vr[8][VW];  // V: keys 2t, 2t + 1, 2t + 8, 2t + 9 of both 16-key tiles; dims VW * 4 * g ..
     int page = -1, next_page = -1;  // of the step in registers, of the one after
     float ks = 0.f, vs = 0.f;
     auto page_of = [&](int u) -> int {
-        if (u >= units) return -1;
+        if (u >= u1) return -1;
         const int p = table[u >> 1];
         return p >= 0 && p < a.n_pages ? p : -1;
     };
@@ -306,10 +403,10 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
             }
         }
     };
-    page = page_of(gw);
-    next_page = page_of(gw + TW);
-    load_k(gw, page);
-    load_v(gw, page);
+    page = page_of(u0);
+    next_page = page_of(u0 + step);
+    load_k(u0, page);
+    load_v(u0, page);
     if (page >= 0) {
         ks = a.kscale[(long)page * a.kv_heads + kvh];
         vs = a.vscale[(long)page * a.kv_heads + kvh];
@@ -377,11 +474,11 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
     }
-    for (int u = gw; u < units; u += TW) {
+    for (int u = u0; u < u1; u += step) {
         const int cur = page;
         const float cks = ks, cvs = vs;
         page = next_page;
-        next_page = page_of(u + 2 * TW);
+        next_page = page_of(u + 2 * step);
         if (page >= 0) {
             ks = a.kscale[(long)page * a.kv_heads + kvh];
             vs = a.vscale[(long)page * a.kv_heads + kvh];
@@ -402,12 +499,13 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
                 for (int k = 0; k < KC * 4; ++k) {
                     const uint32_t w0 = reinterpret_cast<const uint32_t *>(&kr[2 * i][k >> 2])[k & 3];
                     const uint32_t w1 = reinterpret_cast<const uint32_t *>(&kr[2 * i + 1][k >> 2])[k & 3];
-                    const uint32_t a0 = e4m3x2_to_h2(w0), a2 = e4m3x2_to_h2(w0 >> 16);
-                    const uint32_t a1 = e4m3x2_to_h2(w1), a3 = e4m3x2_to_h2(w1 >> 16);
+                    uint32_t a0, a1, a2, a3;
+                    e4m3x4_to_h2x2(w0, a0, a2);
+                    e4m3x4_to_h2x2(w1, a1, a3);
 #pragma unroll
                     for (int n = 0; n < NG; ++n) mma_f16(s[n][i], a0, a1, a2, a3, qb[n][k][0], qb[n][k][1]);
                 }
-            load_k(u + TW, page);
+            load_k(u + step, page);
             // ---- softmax: lane holds heads 2t (e = 0, 2) and 2t + 1 (1, 3), keys g (e < 2) and g + 8
             const int left = (int)min(len - (long)u * kAtKeys, (long)kAtKeys);  // keys that the row sees
             bool move = false;
@@ -493,8 +591,9 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const uint32_t a0 = e4m3x2_to_h2(x[0][j]), a1 = e4m3x2_to_h2(x[0][j] >> 16);
-                        const uint32_t a2 = e4m3x2_to_h2(x[1][j]), a3 = e4m3x2_to_h2(x[1][j] >> 16);
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_to_h2x2(x[0][j], a0, a1);
+                        e4m3x4_to_h2x2(x[1][j], a2, a3);
 #pragma unroll
                         for (int n = 0; n < NG; ++n) mma_f16(acc[n][j], a0, a1, a2, a3, pb[n][i][0], pb[n][i][1]);
                     }
@@ -507,12 +606,12 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
                         for (int e = 0; e < 4; ++e) o[n][2 * w + j][e] = fmaf(acc[n][j][e], cvs, o[n][2 * w + j][e]);
             }
         } else {
-            load_k(u + TW, page);
+            load_k(u + step, page);
         }
-        load_v(u + TW, page);
+        load_v(u + step, page);
     }
 
-    // ---- join the warps, then the cluster's CTAs, then (another launch) the splits
+    // ---- join the warps, then the cluster's CTAs or (another launch) the runs
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
 #pragma unroll
@@ -535,14 +634,15 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
         }
     }
     __syncthreads();
-    const int nh = min(HB, a.G - h0);
-    auto put = [&](int h, int d, float m, float l, float v) {  // the joined part of a cluster
-        const long at = (long)row * a.heads + kvh * a.G + h0 + h;
-        if (a.splits == 1) {
+    const int nh = kEven && u1 <= first ? 0 : min(HB, a.G - h0);  // 0: the run ends before the first step
+    const bool whole = !kEven || (first == 0 && u1 == units);
+    float *part = kEven ? a.part + ((long)blockIdx.x * 2 + (first == 0)) * HB * (D + 2) : nullptr;
+    auto put = [&](int h, int d, float m, float l, float v) {
+        if (whole) {
             reinterpret_cast<T *>(a.out)[(long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d] =
                 from_float<T>(l > 0.f || l != l ? v / l : 0.f);
         } else {
-            float *p = a.part + (at * a.splits + blockIdx.z) * (D + 2);
+            float *p = part + h * (D + 2);
             p[d] = v;
             if (d == 0) {
                 p[D] = m;
@@ -562,17 +662,17 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
             l += s_l[w][h] * f;
             v += s_o[w][h][d] * f;
         }
-        if (a.cluster == 1) {
+        if (kEven || a.cluster == 1) {
             put(h, d, m, l, v);
         } else {
-            s_co[h][d] = v;
+            s_co[kEven ? 0 : h][d] = v;
             if (d == 0) {
                 s_cm[h] = m;
                 s_cl[h] = l;
             }
         }
     }
-    if (a.cluster > 1) {
+    if (!kEven && a.cluster > 1) {
         cluster_sync_all();
         const int share = (nh * D + a.cluster - 1) / a.cluster;
         const int x1 = min(nh * D, (rank + 1) * share);
@@ -585,63 +685,111 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
                 const float mc = ld_cluster(&s_cm[h], c), lc = ld_cluster(&s_cl[h], c);
                 const float f = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - m);
                 l += lc * f;
-                v += ld_cluster(&s_co[h][d], c) * f;
+                v += ld_cluster(&s_co[kEven ? 0 : h][d], c) * f;
             }
             put(h, d, m, l, v);
         }
         cluster_sync_all();  // no CTA leaves while its part is read
     }
+    if (!kEven) return;
+    left_cost -= cut - seg0;
+    if (left_cost <= 0) return;
+    seg0 = 0;
+    if (++hc == HC) {
+        hc = 0;
+        do ++row;
+        while (s_prefix[row] == s_prefix[row + 1]);
+    }
+    __syncthreads();  // the parts in shared memory have been read
+    }
 }
 
-// out = sum over splits of O 2^(m - max), over the sum of l 2^(m - max): one CTA per (head, row)
+// Even shares: out = sum of O 2^(m - max) over the runs that share a (row, head), over the
+// sum of l 2^(m - max).  grid (heads, rows, dim blocks), 256 threads.
 template <typename T, int D>
-__global__ void __launch_bounds__(D * 4) kv8_join_kernel(T *__restrict__ out, long out_rs,
-                                                         const float *__restrict__ part, int heads, int splits) {
-    __shared__ float s_v[4][D], s_l[4][D];
-    const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x % D, q = threadIdx.x / D;
+__global__ void __launch_bounds__(256) kv8_join_kernel(T *__restrict__ out, long out_rs, const float *__restrict__ part,
+                                                       const int *__restrict__ prefix, int rows, int ctas, int G,
+                                                       int chunks, int kv_heads, int HB) {
+    extern __shared__ float s_w[];  // [ctas]: 2^(m - max) of each part
+    __shared__ float s_v[256], s_r[8];
+    const int h = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, dims = D / gridDim.z, groups = 256 / dims;
+    const int d = blockIdx.z * dims + tid % dims, q = tid / dims;
+    const int HC = kv_heads * chunks, hl = h % G, hc = h / G * chunks + hl / HB;
     pdl_wait();
     pdl_trigger();
-    const float *p = part + ((long)row * heads + h) * splits * (D + 2);
+    const int p0 = prefix[row], n = prefix[row + 1] - p0;
+    const long long total = (long long)prefix[rows] * HC;
+    if (n == 0) return;
+    const long long runs = kv8_runs(total, ctas), s0 = (long long)p0 * HC + (long long)hc * n;
+    // the runs with its first and its last step
+    const int c0 = (int)(((s0 + kSegCost + 1) * runs - 1) / total), c1 = (int)(((s0 + n) * runs - 1) / total);
+    if (c0 == c1) return;  // one run had all of it
+    // the first run's part begins with the head group, the others continue it
+    const float *base = part + ((long)c0 * 2 * HB + hl % HB) * (D + 2);
+    const long next = 2l * HB * (D + 2), begins = (long)HB * (D + 2);
+    auto block = [&](float v, bool sum) -> float {  // over the 256 threads
+        v = sum ? warp_sum(v) : warp_max(v);
+        __syncthreads();
+        if ((tid & 31) == 0) s_r[tid >> 5] = v;
+        __syncthreads();
+        v = s_r[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) v = sum ? v + s_r[w] : fmaxf(v, s_r[w]);
+        return v;
+    };
     float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, p[(long)s * (D + 2) + D]);
-    float l = 0.f, v = 0.f;
-    for (int s = q; s < splits; s += 4) {
-        const float *x = p + (long)s * (D + 2);
-        const float mc = x[D], lc = x[D + 1];
-        const float f = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - m);
-        l += lc * f;
-        v += x[d] * f;
+    for (int c = tid; c <= c1 - c0; c += 256) {
+        s_w[c] = base[c * next + (c == 0 ? begins : 0) + D];
+        m = fmaxf(m, s_w[c]);
     }
-    s_v[q][d] = v;
-    s_l[q][d] = l;
+    m = block(m, false);
+    float l = 0.f;
+    for (int c = tid; c <= c1 - c0; c += 256) {
+        const float mc = s_w[c], lc = base[c * next + (c == 0 ? begins : 0) + D + 1];
+        const float f = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - m);
+        s_w[c] = f;
+        l += lc * f;
+    }
+    l = block(l, true);
+    float v = 0.f;
+    if (q == 0) v = base[begins + d] * s_w[0];
+#pragma unroll 8
+    for (int c = 1 + q; c <= c1 - c0; c += groups) v += base[c * next + d] * s_w[c];
+    s_v[tid] = v;
     __syncthreads();
     if (q == 0) {
-        v = (s_v[0][d] + s_v[1][d]) + (s_v[2][d] + s_v[3][d]);
-        l = (s_l[0][d] + s_l[1][d]) + (s_l[2][d] + s_l[3][d]);
+        for (int k = 1; k < groups; ++k) v += s_v[k * dims + tid];
         out[row * out_rs + (long)h * D + d] = from_float<T>(l > 0.f || l != l ? v / l : 0.f);
     }
 }
 
 // How a call's context is shared out.
+constexpr int kEvenMaxRows = 2048;  // their prefix sums lie in shared memory
 struct Kv8Split {
-    int ng, chunks, cluster, splits;
+    int ng, chunks, cluster;
+    int ctas;  // even shares (0: clusters)
 };
-Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int sms) {
+Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sms) {
     Kv8Split s;
     const int G = heads / kv_heads;
     s.ng = G <= 8 ? 1 : 2;
     s.chunks = (G + 8 * s.ng - 1) / (8 * s.ng);
     const long pairs = (long)rows * kv_heads * s.chunks;
     const int units = max_len > 0 ? (max_len - 1) / kAtKeys + 1 : 1;
-    const long ctas = 3l * sms;                                    // that run at a time
+    const int per_sm = s.ng == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);  // CTAs by their registers
+    const long ctas = (long)per_sm * sms;
     const int useful = (units + kAtWarps - 1) / kAtWarps;          // CTAs with a step for every warp
     long want = (ctas + pairs - 1) / pairs;                        // fill the machine
     const int tail = (units + 16 * kAtWarps - 1) / (16 * kAtWarps);  // at most 16 steps per warp
     if (want < tail) want = tail;
     if (want > useful) want = useful;
     s.cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
-    s.splits = want > 8 ? (int)(want / 8) : 1;
+    s.ctas = rows <= kEvenMaxRows && pairs * units > WK_EVENMIN * ctas ? (int)ctas : 0;
     return s;
+}
+long long kv8_ws_bytes(const Kv8Split &s, int rows, int D) {
+    const long long prefix = (4ll * (rows + 1) + 15) / 16 * 16;
+    return s.ctas ? prefix + 4ll * s.ctas * 2 * 8 * s.ng * (D + 2) : 0;
 }
 
 template <typename T, int D> cudaError_t launch_store(const Kv8Store &a, int units, cudaStream_t s) {
@@ -660,42 +808,38 @@ template <typename T, int D> cudaError_t launch_store(const Kv8Store &a, int uni
                : cudaLaunchKernelEx(&cfg, kv8_store_kernel<T, D, false>, a);
 }
 
-template <typename T, int D, int NG>
-cudaError_t launch_attn_ng(const Kv8Attn &a, int rows, cudaStream_t s) {
+template <typename T, int D, int NG> cudaError_t launch_attn_ng(const Kv8Attn &a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.cluster * a.chunks * a.kv_heads, rows, a.splits);
     cfg.blockDim = dim3(kAtWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = g_rt.pdl ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D, NG>, a);
-}
-
-template <typename T, int D> cudaError_t launch_attn(const Kv8Attn &a, int ng, int rows, cudaStream_t s) {
-    cudaError_t e = ng == 1 ? launch_attn_ng<T, D, 1>(a, rows, s) : launch_attn_ng<T, D, 2>(a, rows, s);
-    if (e != cudaSuccess || a.splits == 1) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.heads, rows);
-    cfg.blockDim = dim3(4 * D);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = g_rt.pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = g_rt.pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kv8_join_kernel<T, D>, (T *)a.out, a.out_rs, (const float *)a.part, a.heads,
-                              a.splits);
+    if (a.ctas == 0) {
+        cfg.gridDim = dim3(a.cluster * a.chunks * a.kv_heads, a.rows);
+        cfg.numAttrs = 2;
+        return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D, NG, false>, a);
+    }
+    cfg.gridDim = dim3(a.ctas);
+    cfg.dynamicSmemBytes = 4 * (size_t)(a.rows + 1);
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D, NG, true>, a);
+    if (e != cudaSuccess) return e;
+    // few heads, many parts each: more CTAs per head
+    cfg.gridDim = dim3(a.heads, a.rows, (long)a.heads * a.rows >= 2 * g_rt.num_sms ? 1 : 4);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 4 * (size_t)a.ctas;
+    return cudaLaunchKernelEx(&cfg, kv8_join_kernel<T, D>, (T *)a.out, a.out_rs, (const float *)a.part,
+                              (const int *)a.prefix, a.rows, a.ctas, a.G, a.chunks, a.kv_heads, 8 * NG);
 }
 
-long long kv8_ws_bytes(int rows, int heads, int head_dim, int splits) {
-    return splits > 1 ? 4ll * rows * heads * splits * (head_dim + 2) : 0;
+template <typename T, int D> cudaError_t launch_attn(const Kv8Attn &a, int ng, cudaStream_t s) {
+    return ng == 1 ? launch_attn_ng<T, D, 1>(a, s) : launch_attn_ng<T, D, 2>(a, s);
 }
 
 }  // namespace
@@ -739,7 +883,7 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
 long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim) {
     if (rows < 1 || max_len < 1 || kv_heads < 1 || n_heads < 1 || n_heads % kv_heads || head_dim < 1) return 0;
     const int sms = g_rt.num_sms > 0 ? g_rt.num_sms : 148;
-    return kv8_ws_bytes(rows, n_heads, head_dim, kv8_split(rows, max_len, n_heads, kv_heads, sms).splits);
+    return kv8_ws_bytes(kv8_split(rows, max_len, n_heads, kv_heads, head_dim, sms), rows, head_dim);
 }
 
 int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
@@ -758,11 +902,11 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
         return fail("wk_kv8_attention: row stride below n_heads * head_dim");
     if (((uintptr_t)kpool % 16) || ((uintptr_t)vpool % 16))
         return fail("wk_kv8_attention: pools must be 16-byte aligned");
+    if ((uintptr_t)ws % 16) return fail("wk_kv8_attention: workspace must be 16-byte aligned");
     if (g_rt.device < 0) return fail("wk_kv8_attention: cuda_init() has not been called");
     DeviceGuard guard;
-    Kv8Split sp = kv8_split(rows, max_len, n_heads, kv_heads, g_rt.num_sms);
-    if (!ws || ((uintptr_t)ws % 16)) ws_bytes = 0;
-    while (sp.splits > 1 && kv8_ws_bytes(rows, n_heads, head_dim, sp.splits) > ws_bytes) --sp.splits;
+    Kv8Split sp = kv8_split(rows, max_len, n_heads, kv_heads, head_dim, g_rt.num_sms);
+    if (!ws || ws_bytes < kv8_ws_bytes(sp, rows, head_dim)) sp.ctas = 0;
     Kv8Attn a;
     a.out = out;
     a.out_rs = out_rs;
@@ -785,15 +929,17 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
     a.vec = ((uintptr_t)q % 8) == 0 && q_rs % 4 == 0;
     a.cluster = sp.cluster;
-    a.splits = sp.splits;
-    a.part = (float *)ws;
+    a.rows = rows;
+    a.ctas = sp.ctas;
+    a.prefix = (int *)ws;
+    a.part = (float *)((char *)ws + (4ll * (rows + 1) + 15) / 16 * 16);
     cudaStream_t s = stream();
     cudaError_t e;
     if (dtype == kF16)
-        e = head_dim == 64 ? launch_attn<__half, 64>(a, sp.ng, rows, s) : launch_attn<__half, 128>(a, sp.ng, rows, s);
+        e = head_dim == 64 ? launch_attn<__half, 64>(a, sp.ng, s) : launch_attn<__half, 128>(a, sp.ng, s);
     else
-        e = head_dim == 64 ? launch_attn<__nv_bfloat16, 64>(a, sp.ng, rows, s)
-                           : launch_attn<__nv_bfloat16, 128>(a, sp.ng, rows, s);
+        e = head_dim == 64 ? launch_attn<__nv_bfloat16, 64>(a, sp.ng, s)
+                           : launch_attn<__nv_bfloat16, 128>(a, sp.ng, s);
     if (e != cudaSuccess) return fail("wk_kv8_attention: %s", cudaGetErrorString(e));
     return 0;
 }
