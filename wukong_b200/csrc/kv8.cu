@@ -779,11 +779,11 @@ Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sm
     const int per_sm = s.ng == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);  // CTAs by their registers
     const long ctas = (long)per_sm * sms;
     const int useful = (units + kAtWarps - 1) / kAtWarps;          // CTAs with a step for every warp
-    long want = (ctas + pairs - 1) / pairs;                        // fill the machine
+    long want = ctas / pairs > 0 ? ctas / pairs : 1;               // fill the machine, in one wave
     const int tail = (units + 16 * kAtWarps - 1) / (16 * kAtWarps);  // at most 16 steps per warp
     if (want < tail) want = tail;
     if (want > useful) want = useful;
-    s.cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
+    s.cluster = want >= 8 ? 8 : (int)want;
     s.ctas = rows <= kEvenMaxRows && pairs * units > WK_EVENMIN * ctas ? (int)ctas : 0;
     return s;
 }
