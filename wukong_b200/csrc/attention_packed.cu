@@ -102,6 +102,10 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // blocks that some row of the unit sees in part, warps 10 and 11 set the rows of
 // V behind the sequence's end to zero, and every infinity or NaN inside it too,
 // noting its key and dimension; rows that do see that key get NaN there.
+//
+// Where the units are fewer than half the SMs, a cluster of CTAs takes each, with
+// consecutive shares of its key blocks, and joins O, m and l through distributed
+// shared memory.
 constexpr int kPkThreads = 384;
 constexpr int kPkRegs = 168;  // registers per thread at launch
 constexpr int kPkKeys = 128;  // keys per block
@@ -119,7 +123,7 @@ template <int D> struct PkBars {
     uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
     uint64_t v_raw[4], v_clean[4];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
     uint32_t tmem;
-    int found[4];      // sequence, unit within it
+    int found[6];      // sequence, unit within it, its first query and key rows and their counts
     int units[kPkThreads / 32];
     int bad;           // a non-finite V in a masked block
     int bad_key[D];    // first key that holds one, per dimension
@@ -287,8 +291,31 @@ struct PkArgs {
     int n, q_rows, k_rows, G, GT, chunks, kv_heads;  // heads per K/V head, heads per tile, tiles of heads per K/V head
     float scale_log2;
     int vec;  // out is 16-byte aligned and strided
+    int split;  // CTAs of a cluster, which share a unit's keys
     int *err;
 };
+
+__device__ __forceinline__ void pk_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t pk_peer(const void *p, uint32_t rank) {  // p in the shared memory of CTA `rank`
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float pk_ld_peer(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 pk_ld_peer4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPkThreads, 1)
@@ -326,20 +353,30 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (warp == 9 && lane < 3)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v) : "memory");
     pk_fence_before();
     pdl_wait();
     pdl_trigger();
     // ---- this CTA's unit: the idx-th from the end, so that the longest rows of a long prompt start first
-    const int hb = blockIdx.x % (a.kv_heads * a.chunks), idx = blockIdx.x / (a.kv_heads * a.chunks);
+    const int rank = blockIdx.x % a.split, bid = blockIdx.x / a.split;
+    const int hb = bid % (a.kv_heads * a.chunks), idx = bid / (a.kv_heads * a.chunks);
     const int kvh = hb / a.chunks, chunk = hb % a.chunks;
     const int PT = 128 / a.GT;
     int before = 0;
     for (int i0 = 0; i0 < a.n; i0 += kPkThreads) {
         const int i = a.n - 1 - (i0 + tid);
-        int u = 0;
+        int u = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
         if (i >= 0) {
-            const int q0 = min(max(a.q_starts[i], 0), a.q_rows);
-            u = (min(max(a.q_starts[i + 1], q0), a.q_rows) - q0 + 2 * PT - 1) / (2 * PT);
+            q0 = a.q_starts[i];
+            q1 = a.q_starts[i + 1];
+            k0 = a.k_starts[i];
+            k1 = a.k_starts[i + 1];
+            q0 = min(max(q0, 0), a.q_rows);
+            q1 = min(max(q1, q0), a.q_rows);
+            k0 = min(max(k0, 0), a.k_rows);
+            k1 = min(max(k1, k0), a.k_rows);
+            u = (q1 - q0 + 2 * PT - 1) / (2 * PT);
         }
         int in = u;
 #pragma unroll
@@ -359,6 +396,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if (idx >= first && idx < first + u) {
             B->found[0] = i;
             B->found[1] = u - 1 - (idx - first);
+            B->found[2] = q0;
+            B->found[3] = q1 - q0;
+            B->found[4] = k0;
+            B->found[5] = k1 - k0;
         }
         if (idx < before) break;
     }
@@ -368,19 +409,21 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     const int seq = B->found[0];
     bool ok = true;
     if (seq >= 0) {
-        const int q0 = min(max(a.q_starts[seq], 0), a.q_rows);
-        const int ql = min(max(a.q_starts[seq + 1], q0), a.q_rows) - q0;
-        const int k0 = min(max(a.k_starts[seq], 0), a.k_rows);
-        const int kl = min(max(a.k_starts[seq + 1], k0), a.k_rows) - k0;
-        const int shift = kl - ql;                // query j sees keys 0 .. shift + j
+        const int q0 = B->found[2], ql = B->found[3];
         const int j0 = B->found[1] * 2 * PT;      // first query of the unit
         const int head0 = kvh * a.G + chunk * a.GT;
+        // The unit's last query sees `all` blocks of keys; this CTA's share of them starts at
+        // block `skip`, and from here on keys count from there.
+        const int all = max(0, (B->found[5] - ql + min(j0 + 2 * PT, ql) - 1 + kPkKeys) / kPkKeys);
+        const int share = (all + a.split - 1) / a.split, skip = rank * share;
+        const int k0 = B->found[4] + skip * kPkKeys, kl = B->found[5] - skip * kPkKeys;
+        const int shift = kl - ql;  // query j sees keys 0 .. shift + j
         // blocks of keys that each tile sees (0: none), and the first that some row of the unit sees in part
         auto blocks = [&](int t) -> int {
             const int f = j0 + t * PT;
             if (f >= ql) return 0;
             const int last = shift + min(f + PT, ql) - 1;  // the last key that the tile sees
-            return last < 0 ? 0 : last / kPkKeys + 1;
+            return last < 0 ? 0 : min(last / kPkKeys + 1, share);
         };
         const int n0 = blocks(0), n1 = blocks(1), nb = max(n0, n1);
         const int part = max(0, (shift + j0 + 1) / kPkKeys);  // blocks below this are seen whole by every row
@@ -395,8 +438,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         pk_tma3(smem + L::kQ + t * L::kTile + b * 16384, &maps.q, 64 * b, head0, q0 + j0 + t * PT,
                                 &B->q_full);
                 };
-                mbar_expect_tx(&B->q_full, n1 > 0 ? 2 * qbytes : qbytes);
-                load_q(0);
+                mbar_expect_tx(&B->q_full, n0 > 0 && n1 > 0 ? 2 * qbytes : qbytes);
+                if (n0 > 0) load_q(0);
                 auto raw = [&](int i) -> uint64_t * {
                     return (i & 1) && (i >> 1) >= part ? &B->v_raw[((i >> 1) - part) & 3] : nullptr;
                 };
@@ -517,37 +560,36 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 uint8_t *vb = smem + L::kRing + (size_t)s * L::kTile;
                 const int live = min(kPkKeys, kl - j * kPkKeys);
                 // 16-byte chunks: chunk c of key row r lies at place c ^ (r & 7) of its 128 bytes
-                for (int q = ct; q < kPkKeys * D / 8; q += 64) {
-                    uint4 *p = reinterpret_cast<uint4 *>(vb) + q;
-                    const int r = (q >> 3) & 127;
-                    if (r >= live) {
-                        *p = make_uint4(0, 0, 0, 0);
-                        continue;
-                    }
-                    const uint4 u = *p;
-                    const uint32_t e = PkType<T>::exp_one;
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                constexpr uint32_t e = PkType<T>::exp_one;
+                uint4 *vq = reinterpret_cast<uint4 *>(vb) + ct;
+#pragma unroll 1
+                for (int q = 0; q < kPkKeys * D / 8; q += 8 * 64) {
+                    uint4 u[8];
                     uint32_t hit = 0;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) hit |= (w[x] & 0x7fff7fffu) + e;
-                    if (hit & 0x80008000u) {
-                        const int d0 = (q >> 10) * 64 + ((q & 7) ^ (r & 7)) * 8;
-                        uint32_t z[4];
+                    for (int x = 0; x < 8; ++x) u[x] = vq[q + 64 * x];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t over = ((w[x] & 0x7fff7fffu) + e) & 0x80008000u;
-                            z[x] = w[x];
-                            if (over & 0x8000u) {
-                                z[x] &= 0xffff0000u;
-                                atomicMin(&B->bad_key[d0 + 2 * x], j * kPkKeys + r);
-                            }
-                            if (over & 0x80000000u) {
-                                z[x] &= 0x0000ffffu;
-                                atomicMin(&B->bad_key[d0 + 2 * x + 1], j * kPkKeys + r);
+                    for (int x = 0; x < 8; ++x) {
+                        const int r = ((ct + q + 64 * x) >> 3) & 127;
+                        if (r >= live)
+                            vq[q + 64 * x] = make_uint4(0, 0, 0, 0);
+                        else
+                            hit |= ((u[x].x & 0x7fff7fffu) + e) | ((u[x].y & 0x7fff7fffu) + e) |
+                                   ((u[x].z & 0x7fff7fffu) + e) | ((u[x].w & 0x7fff7fffu) + e);
+                    }
+                    if (hit & 0x80008000u) {  // rare
+                        unsigned short *v = reinterpret_cast<unsigned short *>(vq + q);
+#pragma unroll 1
+                        for (int y = 0; y < 64; ++y) {
+                            const int x = y >> 3, c = ct + q + 64 * x, r = (c >> 3) & 127;
+                            unsigned short *w = v + 64 * 8 * x + (y & 7);
+                            if (r < live && ((*w & 0x7fffu) + (e & 0xffffu)) & 0x8000u) {
+                                *w = 0;
+                                atomicMin(&B->bad_key[(c >> 10) * 64 + ((c & 7) ^ (r & 7)) * 8 + (y & 7)],
+                                          j * kPkKeys + r);
+                                B->bad = 1;
                             }
                         }
-                        *p = make_uint4(z[0], z[1], z[2], z[3]);
-                        B->bad = 1;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -608,9 +650,17 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
                 };
                 // The first half is computed with the maximum so far while this block's is
-                // found, and again in the rare case that the maximum moves.
+                // found, and again in the rare case that the maximum moves (the first block's
+                // is found beforehand).
                 f32x2 sum[2];
                 uint32_t pv[32];
+                if (j == 0) {
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 128; i += 2)
+                        x = fmaxf(x, fmaxf(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])));
+                    m = x;
+                }
                 half(0, true, m, sum, pv);
                 const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 if (mb != mb) l = mb;  // a key that this row sees scores NaN: so does the row
@@ -650,14 +700,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             pk_fence_after();
             // what the clearing warps noted of this tile's blocks
             if (nt > part && ok) pk_wait(&B->v_clean[(nt - 1 - part) & 3], ((nt - 1 - part) >> 2) & 1, a.err, 59);
-            const int h = chunk * a.GT + row % a.GT;
-            const bool mine = row < PT * a.GT && jq < ql && h < a.G && ok;
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
             const bool bad = nt > 0 && B->bad;
-            T *orow = reinterpret_cast<T *>(a.out) + (long)(q0 + jq) * a.out_rs + (long)(kvh * a.G + h) * D;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t ov[32];
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            // 32 values of this row from TMEM
+            auto load_o = [&](int c, uint32_t(&ov)[32]) {
                 if (nt > 0) {
                     pk_ld(o_t + 32 * c, ov);
                     pk_wait_ld();
@@ -666,32 +712,114 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     for (int i = 0; i < 32; ++i) ov[i] = 0;
                 }
                 if (bad) {
+#pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (B->bad_key[32 * c + i] <= lim) ov[i] = 0x7fc00000u;
                 }
-                if (mine) {
-                    uint32_t w[16];
+            };
+            // where row x of tile s goes (null: nowhere)
+            auto row_out = [&](int s, int x) -> T * {
+                const int j = j0 + s * PT + x / a.GT, h = chunk * a.GT + x % a.GT;
+                if (x >= PT * a.GT || j >= ql || h >= a.G || !ok) return nullptr;
+                return reinterpret_cast<T *>(a.out) + (long)(q0 + j) * a.out_rs + (long)(kvh * a.G + h) * D;
+            };
+            if (a.split == 1) {
+                // The warp's rows through the part of the Q tile that they came from (all products
+                // that read it are complete), so that a row is written by consecutive lanes.
+                constexpr int C = D / 8;  // 16-byte chunks per row, chunk c of row r at place c ^ (r & 7)
+                uint4 *buf = reinterpret_cast<uint4 *>(smem + L::kQ + t * L::kTile) + (warp & 3) * 32 * C;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x = l == 0.f ? 0.f : __uint_as_float(ov[2 * i]) * inv;
-                        const float y = l == 0.f ? 0.f : __uint_as_float(ov[2 * i + 1]) * inv;
-                        w[i] = PkType<T>::pack(x, y);
-                    }
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t ov[32], w[16];
+                    load_o(c, ov);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        w[i] = PkType<T>::pack(l == 0.f ? 0.f : __uint_as_float(ov[2 * i]) * inv,
+                                               l == 0.f ? 0.f : __uint_as_float(ov[2 * i + 1]) * inv);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        buf[lane * C + ((4 * c + i) ^ (lane & 7))] =
+                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int x = lane; x < 32 * C; x += 32) {
+                    const int r = x / C, c = x % C;
+                    T *o = row_out(t, (warp & 3) * 32 + r);
+                    if (!o) continue;
+                    const uint4 v = buf[r * C + (c ^ (r & 7))];
                     if (a.vec) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            reinterpret_cast<uint4 *>(orow + 32 * c)[i] =
-                                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                        reinterpret_cast<uint4 *>(o)[c] = v;
                     } else {
-                        unsigned short *o = reinterpret_cast<unsigned short *>(orow + 32 * c);
+                        unsigned short *e = reinterpret_cast<unsigned short *>(o) + 8 * c;
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            o[2 * i] = (unsigned short)w[i];
-                            o[2 * i + 1] = (unsigned short)(w[i] >> 16);
+                        for (int i = 0; i < 4; ++i) {
+                            e[2 * i] = (unsigned short)w[i];
+                            e[2 * i + 1] = (unsigned short)(w[i] >> 16);
                         }
                     }
                 }
+            } else {
+                // O as it stands into the ring, which the products of both tiles have left (16-byte
+                // chunk c of row r at place c ^ (r & 7)), the maxima and sums into the Q tiles' place
+                constexpr int C = D / 4;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                float4 *buf = reinterpret_cast<float4 *>(smem + L::kRing) + (t * 128 + row) * C;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t ov[32];
+                    load_o(c, ov);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        buf[(8 * c + i) ^ (row & 7)] =
+                            make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]),
+                                        __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
+                }
+                float *part_m = reinterpret_cast<float *>(smem + L::kQ), *part_l = part_m + 256;
+                part_m[tid] = m * a.scale_log2;
+                part_l[tid] = l;
+                pk_cluster_sync();
+                // this CTA joins and writes its share of the rows, D / 4 lanes to a row
+                const int rows = (256 + a.split - 1) / a.split, r1 = min(256, (rank + 1) * rows);
+                for (int r = rank * rows + tid / C; r < r1; r += 256 / C) {
+                    T *o = row_out(r >> 7, r & 127);
+                    if (!o) continue;
+                    const int c = tid % C;
+                    float top = -INFINITY;
+                    for (int x = 0; x < a.split; ++x) top = fmaxf(top, pk_ld_peer(pk_peer(&part_m[r], x)));
+                    float sum = 0.f;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int x = 0; x < a.split; ++x) {
+                        const float mx = pk_ld_peer(pk_peer(&part_m[r], x)), lx = pk_ld_peer(pk_peer(&part_l[r], x));
+                        const float4 ox = pk_ld_peer4(
+                            pk_peer(reinterpret_cast<float4 *>(smem + L::kRing) + r * C + (c ^ (r & 7)), x));
+                        const float f = mx == -INFINITY ? (lx != lx ? 1.f : 0.f) : pk_ex2(mx - top);
+                        sum += lx * f;
+                        v.x += ox.x * f;
+                        v.y += ox.y * f;
+                        v.z += ox.z * f;
+                        v.w += ox.w * f;
+                    }
+                    const float is = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+                    const uint32_t w0 = PkType<T>::pack(sum == 0.f ? 0.f : v.x * is, sum == 0.f ? 0.f : v.y * is);
+                    const uint32_t w1 = PkType<T>::pack(sum == 0.f ? 0.f : v.z * is, sum == 0.f ? 0.f : v.w * is);
+                    if (a.vec) {
+                        reinterpret_cast<uint2 *>(o)[c] = make_uint2(w0, w1);
+                    } else {
+                        unsigned short *e = reinterpret_cast<unsigned short *>(o) + 4 * c;
+                        e[0] = (unsigned short)w0;
+                        e[1] = (unsigned short)(w0 >> 16);
+                        e[2] = (unsigned short)w1;
+                        e[3] = (unsigned short)(w1 >> 16);
+                    }
+                }
             }
+        }
+        if (a.split > 1) {
+            __syncwarp();
+            if (warp >= 8) pk_cluster_sync();  // the softmax warps' first
+            pk_cluster_sync();                 // no CTA leaves while its part is read
         }
     }
     pk_fence_before();
@@ -710,7 +838,8 @@ bool pk_map(CUtensorMap *m, const void *base, int dtype, int D, int heads, int r
 
 template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, const PkMaps &maps, int GT, cudaStream_t s) {
     using L = PkLayout<D>;
-    const size_t smem = L::kBars + sizeof(PkBars<D>) + 1024;
+    constexpr size_t smem = L::kBars + sizeof(PkBars<D>) + 1024;
+    static_assert(smem <= 232448, "shared memory of a CTA");
     auto kern = attn_packed_kernel<T, D>;
     static bool configured = false;
     if (!configured) {
@@ -741,17 +870,27 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     // units: ceil(length / (2 PT)) per sequence
     const long long most = (long long)p.q_rows / (2 * PT) + p.n;
     const long long units = most < p.q_rows ? most : p.q_rows;
-    if (units * p.kv_heads * a.chunks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    const long long ctas = units * p.kv_heads * a.chunks;
+    // Few units and long sequences: a cluster to each, with two blocks of keys or more per CTA
+    // (1 prompt of 2000 rows behind 14000, 8 heads over 1: 63 units alone SPLIT_FIGURES).
+    long long split = g_rt.num_sms / ctas, blocks = p.k_rows / ((long long)kPkKeys * p.n);
+    if (split > blocks / 2) split = blocks / 2;
+    a.split = split < 2 ? 1 : split > 8 ? 8 : (int)split;
+    if (ctas * a.split > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * p.kv_heads * a.chunks));
+    cfg.gridDim = dim3((unsigned)(ctas * a.split));
     cfg.blockDim = dim3(kPkThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = g_rt.pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = g_rt.pdl ? 1 : 0;
+    cfg.numAttrs = a.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 
