@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             // what the clearing warps noted of this tile's blocks
             if (nt > part && ok) pk_wait(&B->v_clean[(nt - 1 - part) & 3], ((nt - 1 - part) >> 2) & 1, a.err, 59);
             const bool bad = nt > 0 && B->bad;
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees nothing has O = 0 and l = 0
             // 32 values of this row from TMEM
             auto load_o = [&](int c, uint32_t(&ov)[32]) {
                 if (nt > 0) {
@@ -717,40 +717,41 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         if (B->bad_key[32 * c + i] <= lim) ov[i] = 0x7fc00000u;
                 }
             };
-            // where row x of tile s goes (null: nowhere)
+            // Where row x of tile s goes (null: nowhere).  (The unit is read again from shared
+            // memory, which keeps the loop over the blocks free of what only the end needs.)
             auto row_out = [&](int s, int x) -> T * {
-                const int j = j0 + s * PT + x / a.GT, h = chunk * a.GT + x % a.GT;
-                if (x >= PT * a.GT || j >= ql || h >= a.G || !ok) return nullptr;
-                return reinterpret_cast<T *>(a.out) + (long)(q0 + j) * a.out_rs + (long)(kvh * a.G + h) * D;
+                const int j = B->found[1] * 2 * PT + s * PT + x / a.GT, h = chunk * a.GT + x % a.GT;
+                if (x >= PT * a.GT || j >= B->found[3] || h >= a.G || !ok) return nullptr;
+                return reinterpret_cast<T *>(a.out) + (long)(B->found[2] + j) * a.out_rs + (long)(kvh * a.G + h) * D;
             };
             if (a.split == 1) {
                 // The warp's rows through the part of the Q tile that they came from (all products
                 // that read it are complete), so that a row is written by consecutive lanes.
                 constexpr int C = D / 8;  // 16-byte chunks per row, chunk c of row r at place c ^ (r & 7)
                 uint4 *buf = reinterpret_cast<uint4 *>(smem + L::kQ + t * L::kTile) + (warp & 3) * 32 * C;
+                const T *own = row_out(t, row);  // the row in this lane's registers
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t ov[32], w[16];
                     load_o(c, ov);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        w[i] = PkType<T>::pack(l == 0.f ? 0.f : __uint_as_float(ov[2 * i]) * inv,
-                                               l == 0.f ? 0.f : __uint_as_float(ov[2 * i + 1]) * inv);
+                        w[i] = PkType<T>::pack(__uint_as_float(ov[2 * i]) * inv, __uint_as_float(ov[2 * i + 1]) * inv);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         buf[lane * C + ((4 * c + i) ^ (lane & 7))] =
                             make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 }
                 __syncwarp();
+                const int c = lane % C;  // this lane's chunk of each row that it writes
 #pragma unroll 4
-                for (int x = lane; x < 32 * C; x += 32) {
-                    const int r = x / C, c = x % C;
-                    T *o = row_out(t, (warp & 3) * 32 + r);
-                    if (!o) continue;
+                for (int x = 0; x < C; ++x) {
+                    const int r = x * (32 / C) + lane / C;
+                    T *o = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, (unsigned long long)own, r));
                     const uint4 v = buf[r * C + (c ^ (r & 7))];
-                    if (a.vec) {
+                    if (o && a.vec) {
                         reinterpret_cast<uint4 *>(o)[c] = v;
-                    } else {
+                    } else if (o) {
                         unsigned short *e = reinterpret_cast<unsigned short *>(o) + 8 * c;
                         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -802,8 +803,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         v.w += ox.w * f;
                     }
                     const float is = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                    const uint32_t w0 = PkType<T>::pack(sum == 0.f ? 0.f : v.x * is, sum == 0.f ? 0.f : v.y * is);
-                    const uint32_t w1 = PkType<T>::pack(sum == 0.f ? 0.f : v.z * is, sum == 0.f ? 0.f : v.w * is);
+                    const uint32_t w0 = PkType<T>::pack(v.x * is, v.y * is), w1 = PkType<T>::pack(v.z * is, v.w * is);
                     if (a.vec) {
                         reinterpret_cast<uint2 *>(o)[c] = make_uint2(w0, w1);
                     } else {
