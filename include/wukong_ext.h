@@ -164,9 +164,10 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
  * sequence.  n_heads a multiple of kv_heads; head_dim 64 or 128; dtype of q and
  * out F16 or BF16; strides in elements.  max_len (the longest pos + 1) only
  * chooses how the work is split.  ws [ws_bytes] is the caller's workspace (16-byte
- * aligned), held until the call has run: calls that may overlap need one each;
- * wk_kv8_attention_ws gives the bytes that the best split takes, with fewer (or
- * null and 0) the context is split less. */
+ * aligned): zeroed by the caller before its first use, left fit for the next
+ * call by every call, whatever the sizes; calls that may overlap need one each.
+ * wk_kv8_attention_ws gives the bytes that the best split takes; with fewer (or null
+ * and 0) clusters of CTAs share a row's context and ws is not touched. */
 long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim);
 int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
                      const float *kscale, const float *vscale, int n_pages, const int *block_table, int n_seqs,

@@ -473,7 +473,7 @@ def run_decode(dev, c, max_len, ws=False, extra=0, shift=0, short_ws=None):
     nws = dev.wk_kv8_attention_ws(rows, max_len, c["heads"], c["kv"], c["hd"]) if ws else 0
     if short_ws is not None:
         nws = short_ws
-    pws = up(np.full(max(nws, 16), 0xFF, np.uint8)) if nws else None
+    pws = up(np.zeros(max(nws, 16), np.uint8)) if nws else None
     for _ in range(2):  # the second call finds what the first left in the workspace
         wk.check(dev.wk_kv8_attention(b[0] + 2 * shift, rs, b[1] + 2 * shift, rs, b[2], b[3], b[4], b[5], c["n_pages"],
                                       b[6], c["table"].shape[0], c["table"].shape[1], b[7], b[8], rows, max_len,

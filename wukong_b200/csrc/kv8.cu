@@ -44,35 +44,41 @@ __device__ __forceinline__ float scale_for(float amax) {
     return __uint_as_float((uint32_t)(max(e, kMinScaleExp) + 127) << 23);
 }
 
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a < INFINITY ? a : 0.f;  // infinities saturate, NaN stays NaN; neither sets the scale
-}
+// The 16-bit types order like their bits below the sign.
+template <typename T> struct Kv8Bits {
+    static constexpr uint32_t inf = 0x7c00u;
+    static __device__ __forceinline__ float value(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
+};
+template <> struct Kv8Bits<__nv_bfloat16> {
+    static constexpr uint32_t inf = 0x7f80u;
+    static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b << 16); }
+};
 
 // Eight 16-bit values from p; VEC: p is 16-byte aligned.
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    if (VEC) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const T *t = reinterpret_cast<const T *>(&u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float(p[j]);
-    }
+template <bool VEC> __device__ __forceinline__ uint4 load8(const void *p) {
+    if (VEC) return *reinterpret_cast<const uint4 *>(p);
+    const unsigned short *e = reinterpret_cast<const unsigned short *>(p);
+    return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                      e[6] | (uint32_t)e[7] << 16);
+}
+// Two values, times a power of two -> two e4m3 codes, one rounding.
+template <typename T> __device__ __forceinline__ uint32_t to_e4m3x2(uint32_t w, float inv) {
+    const float lo = Kv8Bits<T>::value(w & 0xffffu), hi = Kv8Bits<T>::value(w >> 16);
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo * inv, hi * inv), __NV_SATFINITE, __NV_E4M3);
 }
 
 // One CTA per (page that the call writes, K/V head): threads 0..127 take K,
-// 128..255 V.  The page's new rows stay in registers between the maximum and
-// the rounding, so each is read once.
+// 128..255 V.  The page's new rows stay in registers, as the 16-bit values that
+// they are, between the maximum and the rounding, so each is read once; their
+// loads are under way while the block table is read.
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Store a) {
+__global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
     constexpr int kChunks = D / 8;               // 8-element chunks per row
     constexpr int kRows = 128 / kChunks;         // rows per pass of 128 threads
     constexpr int kPasses = kKv8Page / kRows;
     __shared__ int s_units[8];
     __shared__ int s_found[5];  // sequence, page index, first row, tokens, first offset
-    __shared__ float s_max[8];
+    __shared__ uint32_t s_max[8];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int unit = blockIdx.x, head = blockIdx.y;
     if (tid == 0) s_found[0] = -1;
@@ -119,43 +125,57 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Store a) {
     __syncthreads();
     if (s_found[0] < 0 || s_found[1] >= a.max_pages) return;
     const int row0 = s_found[2], m = s_found[3], off = s_found[4];
-    const int page = a.table[(long)s_found[0] * a.max_pages + s_found[1]];
-    if (page < 0 || page >= a.n_pages) return;
     const int kv = tid >> 7, t = tid & 127;
     const int c = t % kChunks, r = t / kChunks;
-    const T *x = reinterpret_cast<const T *>(a.x[kv]) + (long)row0 * a.rs[kv] + head * D + c * 8;
-    float v[kPasses][8];
-    float amax = 0.f;
+    const long rs = kv ? a.rs[1] : a.rs[0];
+    const T *x = reinterpret_cast<const T *>(kv ? a.x[1] : a.x[0]) + row0 * rs + head * D + c * 8;
+    float *scales = kv ? a.scale[1] : a.scale[0];
+    uint4 v[kPasses];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const int j = p * kRows + r;
-        if (j < m) {
-            load8<T, VEC>(x + (long)j * a.rs[kv], v[p]);
+        v[p] = j < m ? load8<VEC>(x + j * rs) : make_uint4(0, 0, 0, 0);
+    }
+    const int page = a.table[(long)s_found[0] * a.max_pages + s_found[1]];
+    if (page < 0 || page >= a.n_pages) return;
+    const long ps = (long)page * a.kv_heads + head;
+    const float old = off ? scales[ps] : 0.f;
+    uint32_t top = 0;  // two maxima of magnitudes, as bits
 #pragma unroll
-            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(v[p][e]));
+    for (int p = 0; p < kPasses; ++p) {
+        top = __vmaxu2(top, v[p].x & 0x7fff7fffu);
+        top = __vmaxu2(top, v[p].y & 0x7fff7fffu);
+        top = __vmaxu2(top, v[p].z & 0x7fff7fffu);
+        top = __vmaxu2(top, v[p].w & 0x7fff7fffu);
+    }
+    if (__vcmpgeu2(top, Kv8Bits<T>::inf * 0x10001u)) {
+        // infinities saturate and NaN stays NaN, but neither sets the scale
+        top = 0;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t b = w[e] & 0x7fff7fffu;
+                top = __vmaxu2(top, b & ~__vcmpgeu2(b, Kv8Bits<T>::inf * 0x10001u));
+            }
         }
     }
-    const long ps = (long)page * a.kv_heads + head;
-    const float old = off ? a.scale[kv][ps] : 0.f;
-    amax = warp_max(amax);
-    if (lane == 0) s_max[wid] = amax;
+    top = max(top & 0xffffu, top >> 16);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s_max[wid] = top;
     __syncthreads();
-    amax = fmaxf(fmaxf(s_max[4 * kv], s_max[4 * kv + 1]), fmaxf(s_max[4 * kv + 2], s_max[4 * kv + 3]));
-    const float scale = fmaxf(old, scale_for(amax));
+    top = max(max(s_max[4 * kv], s_max[4 * kv + 1]), max(s_max[4 * kv + 2], s_max[4 * kv + 3]));
+    const float scale = fmaxf(old, scale_for(Kv8Bits<T>::value(top)));
     const float inv = 1.0f / scale;  // a power of two: exact
-    uint8_t *dst = a.pool[kv] + (size_t)ps * (kKv8Page * D);
+    uint8_t *dst = (kv ? a.pool[1] : a.pool[0]) + (size_t)ps * (kKv8Page * D);
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const int j = p * kRows + r;
-        if (j < m) {
-            uint2 o;
-            __nv_fp8x2_storage_t *w = reinterpret_cast<__nv_fp8x2_storage_t *>(&o);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[e] = __nv_cvt_float2_to_fp8x2(make_float2(v[p][2 * e] * inv, v[p][2 * e + 1] * inv), __NV_SATFINITE,
-                                                __NV_E4M3);
-            *reinterpret_cast<uint2 *>(dst + (off + j) * D + c * 8) = o;
-        }
+        if (j < m)
+            *reinterpret_cast<uint2 *>(dst + (off + j) * D + c * 8) =
+                make_uint2(to_e4m3x2<T>(v[p].x, inv) | to_e4m3x2<T>(v[p].y, inv) << 16,
+                           to_e4m3x2<T>(v[p].z, inv) | to_e4m3x2<T>(v[p].w, inv) << 16);
     }
     if (off && scale != old) {  // the tokens that the page held move to the new scale
         const float ratio = old * inv;
@@ -166,7 +186,7 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Store a) {
             *w = __nv_cvt_float2_to_fp8x2(make_float2(f.x * ratio, f.y * ratio), __NV_SATFINITE, __NV_E4M3);
         }
     }
-    if (t == 0) a.scale[kv][ps] = scale;
+    if (t == 0) scales[ps] = scale;
 }
 
 // ------------------------------------------------------------------ attention
@@ -186,8 +206,9 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Store a) {
 //             (m, l, O) through distributed shared memory: one launch
 //   even      the steps of all rows and K/V heads, one after the other, are cut into as
 //             many equal runs as CTAs fit on the GPU; a run that ends inside a
-//             (row, K/V head) leaves its part in the caller's workspace, and a second
-//             launch joins those
+//             (row, K/V head) leaves its part in the caller's workspace, and the last of
+//             them to arrive joins the parts in their order (a second launch does, where
+//             they are many)
 constexpr int kAtWarps = 4;
 #ifndef WK_EVENMIN
 #define WK_EVENMIN 8
@@ -211,8 +232,10 @@ struct Kv8Attn {
     int rows;
     int cluster;   // CTAs that share a (row, K/V head)
     int ctas;      // even shares: CTAs of the launch
+    int *tickets;  // even shares: [kTickets] arrivals of a head group's parts, at the run with its first step; zero
+                   // between calls.  Null: a second launch joins the parts.
     int *prefix;   // even shares: [rows + 1] cost of the rows before each, per head group (written by CTA 0)
-    float *part;   // even shares: [ctas][2][8 NG][D + 2]: O, m, l of a run's part of a head group
+    float *part;   // even shares: [ctas][2][8 NG][D + 4]: O, m, l of a run's part of a head group
 };
 
 // Even shares: a (row, head group) of n steps costs n + kSegCost, the latencies of
@@ -223,6 +246,11 @@ struct Kv8Attn {
 #define WK_SEGCOST 8
 #endif
 constexpr int kSegCost = WK_SEGCOST;
+constexpr int kTickets = 4096;  // at most so many CTAs
+// the run that has place x of the cost
+__device__ __forceinline__ int kv8_owner(long long x, long long runs, long long total) {
+    return (int)(((x + 1) * runs - 1) / total);
+}
 __device__ __forceinline__ long long kv8_runs(long long total, int ctas) {
     const long long most = (total + kSegCost + 7) / (kSegCost + 8);
     return most < ctas ? (most > 0 ? most : 1) : ctas;
@@ -281,6 +309,7 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
     constexpr int KC = D / 64;       // 16-byte pieces of a K row per lane
     constexpr int MT = D / 16;       // 16-dim tiles of O
     constexpr int VW = D / 32;       // 32-bit words of a V row per lane
+    constexpr int kPart = D + 4;     // floats of a part: O, m, l, 2 unused
     __shared__ float s_o[kAtWarps][HB][D];
     __shared__ float s_m[kAtWarps][HB], s_l[kAtWarps][HB];
     __shared__ float s_co[kEven ? 1 : HB][D], s_cm[HB], s_cl[HB];  // this CTA's part, read by the cluster
@@ -299,6 +328,7 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
     int u0, u1, step;         // this warp's steps of the segment: u0, u0 + step, ... below u1
     int seg0 = 0;              // even shares: where the run stands in the head group's cost
     long long left_cost = 0;   // even shares: what is left of this CTA's run
+    long long total = 0, runs = 0;
     if (kEven) {
         // cost of the rows before each
         int base = 0;
@@ -325,14 +355,15 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
         }
         if (tid == 0) s_prefix[a.rows] = base;
         __syncthreads();
-        if (blockIdx.x == 0)
+        if (blockIdx.x == 0 && !a.tickets)
             for (int r = tid; r <= a.rows; r += kAtWarps * 32) a.prefix[r] = s_prefix[r];
         // rows that see nothing
         for (int r = blockIdx.x; r < a.rows; r += a.ctas)
             if (s_prefix[r] == s_prefix[r + 1])
                 for (int x = tid; x < a.heads * D; x += kAtWarps * 32)
                     reinterpret_cast<T *>(a.out)[(long)r * a.out_rs + x] = from_float<T>(0.f);
-        const long long total = (long long)base * HC, runs = kv8_runs(total, a.ctas);
+        total = (long long)base * HC;
+        runs = kv8_runs(total, a.ctas);
         if (total == 0 || blockIdx.x >= runs) return;
         const long long b0 = blockIdx.x * total / runs;
         left_cost = (blockIdx.x + 1) * total / runs - b0;
@@ -636,13 +667,13 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
     __syncthreads();
     const int nh = kEven && u1 <= first ? 0 : min(HB, a.G - h0);  // 0: the run ends before the first step
     const bool whole = !kEven || (first == 0 && u1 == units);
-    float *part = kEven ? a.part + ((long)blockIdx.x * 2 + (first == 0)) * HB * (D + 2) : nullptr;
+    float *part = kEven ? a.part + ((long)blockIdx.x * 2 + (first == 0)) * HB * kPart : nullptr;
     auto put = [&](int h, int d, float m, float l, float v) {
         if (whole) {
             reinterpret_cast<T *>(a.out)[(long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d] =
                 from_float<T>(l > 0.f || l != l ? v / l : 0.f);
         } else {
-            float *p = part + h * (D + 2);
+            float *p = part + h * kPart;
             p[d] = v;
             if (d == 0) {
                 p[D] = m;
@@ -692,6 +723,73 @@ __global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a
         cluster_sync_all();  // no CTA leaves while its part is read
     }
     if (!kEven) return;
+    if (nh > 0 && !whole && a.tickets) {
+        __shared__ int s_last;
+        const int n = units + kSegCost;
+        const long long s0 = (long long)s_prefix[row] * HC + (long long)hc * n;
+        const int c0 = kv8_owner(s0 + kSegCost, runs, total), c1 = kv8_owner(s0 + n - 1, runs, total);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            s_last = atomicAdd(&a.tickets[c0], 1) == c1 - c0;
+            if (s_last) a.tickets[c0] = 0;
+        }
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            // part 0 begins the head group in run c0, the others continue it
+            auto at = [&](int c) { return a.part + ((long)(c0 + c) * 2 + (c == 0)) * HB * kPart; };
+            const int parts = c1 - c0 + 1;
+            constexpr int NV = HB * D / 4 / (kAtWarps * 32);  // float4 outputs per thread
+            float4 v[NV];
+            float m[NV], l[NV];
+#pragma unroll
+            for (int y = 0; y < NV; ++y) {
+                v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                m[y] = -INFINITY;
+                l[y] = 0.f;
+            }
+            float(*s_pm)[2][HB] = reinterpret_cast<float(*)[2][HB]>(&s_o[0][0][0]);  // [32 parts][m, l][head]
+            for (int cb = 0; cb < parts; cb += 32) {
+                const int nc = min(32, parts - cb);
+                __syncthreads();
+                for (int x = tid; x < nc * 2 * HB; x += kAtWarps * 32) {
+                    const int c = x / (2 * HB), k = x / HB & 1, h = x % HB;
+                    s_pm[c][k][h] = h < nh ? __ldcg(at(cb + c) + h * kPart + D + k) : 0.f;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int y = 0; y < NV; ++y) {
+                    const int x = tid + y * kAtWarps * 32, h = x / (D / 4), d = x % (D / 4) * 4;
+                    float mn = m[y];
+                    for (int c = 0; c < nc; ++c) mn = fmaxf(mn, s_pm[c][0][h]);
+                    const float f = m[y] == -INFINITY ? 1.f : ex2(m[y] - mn);  // with m = -inf, v and l are 0
+                    m[y] = mn;
+                    l[y] *= f;
+                    v[y].x *= f, v[y].y *= f, v[y].z *= f, v[y].w *= f;
+#pragma unroll 4
+                    for (int c = 0; c < nc; ++c) {
+                        const float4 o = __ldcg(reinterpret_cast<const float4 *>(at(cb + c) + h * kPart + d));
+                        const float mc = s_pm[c][0][h], lc = s_pm[c][1][h];
+                        const float fc = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - mn);
+                        l[y] += lc * fc;
+                        v[y].x += o.x * fc, v[y].y += o.y * fc, v[y].z += o.z * fc, v[y].w += o.w * fc;
+                    }
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < NV; ++y) {
+                const int x = tid + y * kAtWarps * 32, h = x / (D / 4), d = x % (D / 4) * 4;
+                if (h >= nh) continue;
+                const float inv = l[y] > 0.f || l[y] != l[y] ? 1.f / l[y] : 0.f;
+                T *o = reinterpret_cast<T *>(a.out) + (long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d;
+                o[0] = from_float<T>(v[y].x * inv);
+                o[1] = from_float<T>(v[y].y * inv);
+                o[2] = from_float<T>(v[y].z * inv);
+                o[3] = from_float<T>(v[y].w * inv);
+            }
+        }
+    }
     left_cost -= cut - seg0;
     if (left_cost <= 0) return;
     seg0 = 0;
@@ -710,7 +808,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) kv8_join_kernel(T *__restrict__ out, long out_rs, const float *__restrict__ part,
                                                        const int *__restrict__ prefix, int rows, int ctas, int G,
                                                        int chunks, int kv_heads, int HB) {
-    extern __shared__ float s_w[];  // [ctas]: 2^(m - max) of each part
+    extern __shared__ float s_w[];  // [2][ctas]: m, then 2^(m - max), and l of each part
     __shared__ float s_v[256], s_r[8];
     const int h = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, dims = D / gridDim.z, groups = 256 / dims;
     const int d = blockIdx.z * dims + tid % dims, q = tid / dims;
@@ -722,11 +820,11 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(T *__restrict__ out, long
     if (n == 0) return;
     const long long runs = kv8_runs(total, ctas), s0 = (long long)p0 * HC + (long long)hc * n;
     // the runs with its first and its last step
-    const int c0 = (int)(((s0 + kSegCost + 1) * runs - 1) / total), c1 = (int)(((s0 + n) * runs - 1) / total);
+    const int c0 = kv8_owner(s0 + kSegCost, runs, total), c1 = kv8_owner(s0 + n - 1, runs, total);
     if (c0 == c1) return;  // one run had all of it
     // the first run's part begins with the head group, the others continue it
-    const float *base = part + ((long)c0 * 2 * HB + hl % HB) * (D + 2);
-    const long next = 2l * HB * (D + 2), begins = (long)HB * (D + 2);
+    const float *base = part + ((long)c0 * 2 * HB + hl % HB) * (D + 4);
+    const long next = 2l * HB * (D + 4), begins = (long)HB * (D + 4);
     auto block = [&](float v, bool sum) -> float {  // over the 256 threads
         v = sum ? warp_sum(v) : warp_max(v);
         __syncthreads();
@@ -739,13 +837,15 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(T *__restrict__ out, long
     };
     float m = -INFINITY;
     for (int c = tid; c <= c1 - c0; c += 256) {
-        s_w[c] = base[c * next + (c == 0 ? begins : 0) + D];
+        const float *p = base + c * next + (c == 0 ? begins : 0) + D;
+        s_w[c] = p[0];
+        s_w[ctas + c] = p[1];
         m = fmaxf(m, s_w[c]);
     }
     m = block(m, false);
     float l = 0.f;
     for (int c = tid; c <= c1 - c0; c += 256) {
-        const float mc = s_w[c], lc = base[c * next + (c == 0 ? begins : 0) + D + 1];
+        const float mc = s_w[c], lc = s_w[ctas + c];
         const float f = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : ex2(mc - m);
         s_w[c] = f;
         l += lc * f;
@@ -768,6 +868,7 @@ constexpr int kEvenMaxRows = 2048;  // their prefix sums lie in shared memory
 struct Kv8Split {
     int ng, chunks, cluster;
     int ctas;  // even shares (0: clusters)
+    bool wide;  // even shares: more than 16 parts to a head group, which a second launch joins
 };
 Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sms) {
     Kv8Split s;
@@ -784,12 +885,13 @@ Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sm
     if (want < tail) want = tail;
     if (want > useful) want = useful;
     s.cluster = want >= 8 ? 8 : (int)want;
+    s.wide = pairs * 16 < ctas;
     s.ctas = rows <= kEvenMaxRows && pairs * units > WK_EVENMIN * ctas ? (int)ctas : 0;
     return s;
 }
 long long kv8_ws_bytes(const Kv8Split &s, int rows, int D) {
     const long long prefix = (4ll * (rows + 1) + 15) / 16 * 16;
-    return s.ctas ? prefix + 4ll * s.ctas * 2 * 8 * s.ng * (D + 2) : 0;
+    return s.ctas ? 4ll * kTickets + prefix + 4ll * s.ctas * 2 * 8 * s.ng * (D + 4) : 0;
 }
 
 template <typename T, int D> cudaError_t launch_store(const Kv8Store &a, int units, cudaStream_t s) {
@@ -829,11 +931,10 @@ template <typename T, int D, int NG> cudaError_t launch_attn_ng(const Kv8Attn &a
     cfg.dynamicSmemBytes = 4 * (size_t)(a.rows + 1);
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D, NG, true>, a);
-    if (e != cudaSuccess) return e;
-    // few heads, many parts each: more CTAs per head
-    cfg.gridDim = dim3(a.heads, a.rows, (long)a.heads * a.rows >= 2 * g_rt.num_sms ? 1 : 4);
+    if (e != cudaSuccess || a.tickets) return e;
+    cfg.gridDim = dim3(a.heads, a.rows, (long)a.heads * a.rows >= g_rt.num_sms / 2 ? 4 : 8);
     cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 4 * (size_t)a.ctas;
+    cfg.dynamicSmemBytes = 8 * (size_t)a.ctas;
     return cudaLaunchKernelEx(&cfg, kv8_join_kernel<T, D>, (T *)a.out, a.out_rs, (const float *)a.part,
                               (const int *)a.prefix, a.rows, a.ctas, a.G, a.chunks, a.kv_heads, 8 * NG);
 }
@@ -931,8 +1032,9 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     a.cluster = sp.cluster;
     a.rows = rows;
     a.ctas = sp.ctas;
-    a.prefix = (int *)ws;
-    a.part = (float *)((char *)ws + (4ll * (rows + 1) + 15) / 16 * 16);
+    a.tickets = sp.wide ? nullptr : (int *)ws;
+    a.prefix = (int *)ws + kTickets;
+    a.part = (float *)((char *)ws + 4ll * kTickets + (4ll * (rows + 1) + 15) / 16 * 16);
     cudaStream_t s = stream();
     cudaError_t e;
     if (dtype == kF16)
