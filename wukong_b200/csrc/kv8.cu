@@ -215,6 +215,9 @@ constexpr int kAtWarps = 4;
 #endif
 constexpr int kAtKeys = 32;  // keys per warp and step
 
+// CTAs that an SM holds, by their registers.
+constexpr int kv8_per_sm(int ng, int D) { return ng == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2); }
+
 struct Kv8Attn {
     void *out;
     long out_rs;
@@ -304,7 +307,7 @@ template <> struct Kv8Q<__nv_bfloat16> {
 
 // grid: clusters (cluster * chunks * kv_heads, rows); even shares (ctas)
 template <typename T, int D, int NG, bool kEven>
-__global__ void __launch_bounds__(kAtWarps * 32) kv8_attn_kernel(const Kv8Attn a) {
+__global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_kernel(const Kv8Attn a) {
     constexpr int HB = 8 * NG;       // heads per CTA
     constexpr int KC = D / 64;       // 16-byte pieces of a K row per lane
     constexpr int MT = D / 16;       // 16-dim tiles of O
@@ -877,8 +880,7 @@ Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sm
     s.chunks = (G + 8 * s.ng - 1) / (8 * s.ng);
     const long pairs = (long)rows * kv_heads * s.chunks;
     const int units = max_len > 0 ? (max_len - 1) / kAtKeys + 1 : 1;
-    const int per_sm = s.ng == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);  // CTAs by their registers
-    const long ctas = (long)per_sm * sms;
+    const long ctas = (long)kv8_per_sm(s.ng, D) * sms;
     const int useful = (units + kAtWarps - 1) / kAtWarps;          // CTAs with a step for every warp
     long want = ctas / pairs > 0 ? ctas / pairs : 1;               // fill the machine, in one wave
     const int tail = (units + 16 * kAtWarps - 1) / (16 * kAtWarps);  // at most 16 steps per warp
