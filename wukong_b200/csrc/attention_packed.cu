@@ -83,12 +83,9 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 }
 
 // ------------------------------------------------------------------ tcgen05 kernel
-// A unit is 2 tiles of 128 query rows of one K/V head, a tile being PT = 128 / G
-// positions times the G heads of the group (heads inner), so that a K/V tile
-// loaded once serves all of them.  One CTA per SM works through units; it takes
-// the next one over from the grid's CTAs that have not started yet (cluster launch
-// control), so that Q, K and V of a unit are on their way while the one before it
-// ends and the longest units, which come first in the grid, are not bunched.  Per block of 128 keys and tile t:
+// A CTA takes one unit: 2 tiles of 128 query rows of one K/V head, a tile being
+// PT = 128 / G positions times the G heads of the group (heads inner), so that a
+// K/V tile loaded once serves all of them.  Per block of 128 keys and tile t:
 //   S_t = Q_t K^T  (TMEM, fp32)       P_t = exp2(c (S_t - m))  (16 bits, over S_t in TMEM)
 //   O_t += P_t V   (TMEM, fp32)       l_t += row sums of P_t before rounding
 // m is a maximum that is moved, and O_t and l_t scaled, only when it falls more
@@ -97,13 +94,12 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 //   warps 0-3, 4-7   softmax of tile 0, tile 1 (one thread per row), epilogue
 //   warp 8           issues the tcgen05.mma
 //   warp 9           TMA: Q, then K and V blocks through a ring
-//   warp 10          clears what masked keys of V hold (see below)
-//   warp 11          finds the units
+//   warps 10, 11     clear what masked keys of V hold (see below)
 // While one tile's softmax runs on the CUDA cores, the tensor cores run the
 // other tile's P V and its next Q K^T.
 //
 // A masked key has p = 0, but 0 * NaN is NaN in a product of tiles.  So in the
-// blocks that some row of the unit sees in part, warp 10 sets the rows of
+// blocks that some row of the unit sees in part, warps 10 and 11 set the rows of
 // V behind the sequence's end to zero, and every infinity or NaN inside it too,
 // noting its key and dimension; rows that do see that key get NaN there.
 //
@@ -116,31 +112,21 @@ constexpr int kPkKeys = 128;  // keys per block
 
 template <int D> struct PkLayout {
     static constexpr int kTile = 128 * D * 2;                 // bytes of a Q tile or a K / V block
-    static constexpr int kStages = D == 128 ? 4 : 8;
+    static constexpr int kStages = D == 128 ? 5 : 8;
     static constexpr size_t kQ = 0;
     static constexpr size_t kRing = 2 * (size_t)kTile;
-    static constexpr size_t kOut = kRing + (size_t)kStages * kTile;  // 4 KB per softmax warp
-    static constexpr size_t kBars = kOut + 8 * 4096;
-};
-
-struct PkUnit {
-    int valid;
-    int q0, ql, k0, kl;  // the sequence's first rows and their counts
-    int j0;              // first query of the unit
-    int kvh, chunk;
+    static constexpr size_t kBars = kRing + (size_t)kStages * kTile;
 };
 
 template <int D> struct PkBars {
-    uint64_t kv_full[PkLayout<D>::kStages], kv_empty[PkLayout<D>::kStages];
-    uint64_t q_full[2], q_empty[2];
+    uint64_t q_full, kv_full[PkLayout<D>::kStages], kv_empty[PkLayout<D>::kStages];
     uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-    uint64_t v_raw[8], v_clean[8];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
-    uint64_t u_full[2], u_empty[2], u_want, u_got;
-    uint4 claim;                    // the answer of cluster launch control
-    PkUnit unit[2];
+    uint64_t v_raw[4], v_clean[4];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
     uint32_t tmem;
-    int bad[2];                     // a non-finite V in a masked block of the unit
-    int bad_key[2][D];              // first key that holds one, per dimension
+    int found[6];      // sequence, unit within it, its first query and key rows and their counts
+    int units[kPkThreads / 32];
+    int bad;           // a non-finite V in a masked block
+    __align__(16) int bad_key[D];  // first key that holds one, per dimension
 };
 
 struct PkMaps {
@@ -342,28 +328,26 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in the whole warp
     if (tid == 0) {
+        mbar_init(&B->q_full, 1);
         for (int i = 0; i < ST; ++i) {
             mbar_init(&B->kv_full[i], 1);
             mbar_init(&B->kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&B->q_full[i], 1);
-            mbar_init(&B->q_empty[i], 1);
             mbar_init(&B->s_full[i], 1);
             mbar_init(&B->p_half[i], 128);
             mbar_init(&B->p_full[i], 128);
             mbar_init(&B->o_full[i], 1);
-            mbar_init(&B->u_full[i], 1);
-            mbar_init(&B->u_empty[i], 11);  // 8 softmax warps, warps 8, 9 and 10
         }
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&B->v_raw[i], 1);
-            mbar_init(&B->v_clean[i], 32);
+            mbar_init(&B->v_clean[i], 64);
         }
-        mbar_init(&B->u_want, 1);
-        mbar_init(&B->u_got, 1);
         mbar_fence_init();
+        B->found[0] = -1;
+        B->bad = 0;
     }
+    for (int i = tid; i < D; i += kPkThreads) B->bad_key[i] = 0x7fffffff;
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem))
                      : "memory");
@@ -374,211 +358,121 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     pk_fence_before();
     pdl_wait();
     pdl_trigger();
+    // ---- this CTA's unit: the idx-th from the end, so that the longest rows of a long prompt start first
+    const int rank = blockIdx.x % a.split, bid = blockIdx.x / a.split;
+    const int hb = bid % (a.kv_heads * a.chunks), idx = bid / (a.kv_heads * a.chunks);
+    const int kvh = hb / a.chunks, chunk = hb % a.chunks;
+    const int PT = 128 / a.GT;
+    int before = 0;
+    for (int i0 = 0; i0 < a.n; i0 += kPkThreads) {
+        const int i = a.n - 1 - (i0 + tid);
+        int u = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+        if (i >= 0) {
+            q0 = a.q_starts[i];
+            q1 = a.q_starts[i + 1];
+            k0 = a.k_starts[i];
+            k1 = a.k_starts[i + 1];
+            q0 = min(max(q0, 0), a.q_rows);
+            q1 = min(max(q1, q0), a.q_rows);
+            k0 = min(max(k0, 0), a.k_rows);
+            k1 = min(max(k1, k0), a.k_rows);
+            u = (q1 - q0 + 2 * PT - 1) / (2 * PT);
+        }
+        int in = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, in, o);
+            if (lane >= o) in += v;
+        }
+        __syncthreads();
+        if (lane == 31) B->units[warp] = in;
+        __syncthreads();
+        int first = before + in - u;
+#pragma unroll
+        for (int w = 0; w < kPkThreads / 32; ++w) {
+            if (w < warp) first += B->units[w];
+            before += B->units[w];
+        }
+        if (idx >= first && idx < first + u) {
+            B->found[0] = i;
+            B->found[1] = u - 1 - (idx - first);
+            B->found[2] = q0;
+            B->found[3] = q1 - q0;
+            B->found[4] = k0;
+            B->found[5] = k1 - k0;
+        }
+        if (idx < before) break;
+    }
     __syncthreads();
     pk_fence_after();
     const uint32_t tmem = B->tmem;
-    const int rank = blockIdx.x % a.split;
-    const int PT = 128 / a.GT;
+    const int seq = B->found[0];
     bool ok = true;
-    // What a unit means for this CTA.  Its last query sees `all` blocks of keys; the share of
-    // this CTA of the cluster starts at block rank * share, and keys count from there.
-    struct View {
-        int q0, ql, k0, kl, j0, shift, n0, n1, nb, part;
-    };
-    auto view = [&](int slot) -> View {
-        const PkUnit &u = B->unit[slot];
-        View v;
-        v.q0 = u.q0;
-        v.ql = u.ql;
-        v.j0 = u.j0;
-        const int all = max(0, (u.kl - u.ql + min(u.j0 + 2 * PT, u.ql) - 1 + kPkKeys) / kPkKeys);
+    if (seq >= 0) {
+        const int q0 = B->found[2], ql = B->found[3];
+        const int j0 = B->found[1] * 2 * PT;      // first query of the unit
+        const int head0 = kvh * a.G + chunk * a.GT;
+        // The unit's last query sees `all` blocks of keys; this CTA's share of them starts at
+        // block `skip`, and from here on keys count from there.
+        const int all = max(0, (B->found[5] - ql + min(j0 + 2 * PT, ql) - 1 + kPkKeys) / kPkKeys);
         const int share = (all + a.split - 1) / a.split, skip = rank * share;
-        v.k0 = u.k0 + skip * kPkKeys;
-        v.kl = u.kl - skip * kPkKeys;
-        v.shift = v.kl - v.ql;  // query j sees keys 0 .. shift + j
+        const int k0 = B->found[4] + skip * kPkKeys, kl = B->found[5] - skip * kPkKeys;
+        const int shift = kl - ql;  // query j sees keys 0 .. shift + j
         // blocks of keys that each tile sees (0: none), and the first that some row of the unit sees in part
         auto blocks = [&](int t) -> int {
-            const int f = u.j0 + t * PT;
-            if (f >= u.ql) return 0;
-            const int last = v.shift + min(f + PT, u.ql) - 1;  // the last key that the tile sees
+            const int f = j0 + t * PT;
+            if (f >= ql) return 0;
+            const int last = shift + min(f + PT, ql) - 1;  // the last key that the tile sees
             return last < 0 ? 0 : min(last / kPkKeys + 1, share);
         };
-        v.n0 = blocks(0);
-        v.n1 = blocks(1);
-        v.nb = max(v.n0, v.n1);
-        v.part = max(0, (v.shift + u.j0 + 1) / kPkKeys);  // blocks below this are seen whole by every row
-        return v;
-    };
-    // The u-th unit of this CTA; false: none is left (or a wait gave up).
-    auto begin = [&](int u) -> bool {
-        ok = ok && pk_wait(&B->u_full[u & 1], (u >> 1) & 1, a.err, 61);
-        return ok && B->unit[u & 1].valid;
-    };
-    // registers: 256 softmax threads x 216 + 128 x 72 = the launch's 384 x 168
-    if (warp >= 8) {
+        const int n0 = blocks(0), n1 = blocks(1), nb = max(n0, n1);
+        const int part = max(0, (shift + j0 + 1) / kPkKeys);  // blocks below this are seen whole by every row
+        // registers: 256 softmax threads x 216 + 128 x 72 = the launch's 384 x 168
+        if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 11) {
-            // ---- units, from the last of the grid's order (sequences and positions descending), so that
-            // the longest rows of a long prompt start first.  Lane i looks at sequence n - 1 - (i0 + i).
-            const int HC = a.kv_heads * a.chunks;
-            int claims = 0, i0 = 0, before = 0, total = 0, first = 0, units = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-            auto look = [&]() {
-                const int i = a.n - 1 - (i0 + lane);
-                q0 = q1 = k0 = k1 = 0;
-                if (i >= 0) {
-                    q0 = a.q_starts[i];
-                    q1 = a.q_starts[i + 1];
-                    k0 = a.k_starts[i];
-                    k1 = a.k_starts[i + 1];
-                    q0 = min(max(q0, 0), a.q_rows);
-                    q1 = min(max(q1, q0), a.q_rows);
-                    k0 = min(max(k0, 0), a.k_rows);
-                    k1 = min(max(k1, k0), a.k_rows);
-                }
-                units = (q1 - q0 + 2 * PT - 1) / (2 * PT);
-                int in = units;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_up_sync(0xffffffffu, in, o);
-                    if (lane >= o) in += v;
-                }
-                first = before + in - units;
-                total = __shfl_sync(0xffffffffu, before + in, 31);
-            };
-            look();
-            int work = blockIdx.x / a.split;
-            bool more = true;
-            for (int u = 0; ok; ++u) {
-                if (u >= 2) ok = __all_sync(0xffffffffu, pk_wait(&B->u_empty[u & 1], ((u >> 1) - 1) & 1, a.err, 62));
-                bool valid = false;
-                while (ok && more) {
-                    if (work >= 0) {
-                        const int idx = work / HC, hb = work % HC;
-                        if (idx < before) {
-                            i0 = before = 0;
-                            look();
-                        }
-                        while (idx >= total && i0 + 32 < a.n) {
-                            before = total;
-                            i0 += 32;
-                            look();
-                        }
-                        valid = idx < total;
-                        if (idx >= first && idx < first + units) {
-                            PkUnit &x = B->unit[u & 1];
-                            x.q0 = q0;
-                            x.ql = q1 - q0;
-                            x.k0 = k0;
-                            x.kl = k1 - k0;
-                            x.j0 = (units - 1 - (idx - first)) * 2 * PT;
-                            x.kvh = hb / a.chunks;
-                            x.chunk = hb % a.chunks;
-                        }
-                        work = -1;
-                        if (valid) break;
-                    }
-                    if (a.split > 1) {  // a cluster takes one unit
-                        more = false;
+        if (warp == 9) {
+            if (nb > 0 && pk_elect()) {
+                const uint32_t qbytes = (uint32_t)(PT * a.GT) * D * 2;
+                auto load_q = [&](int t) {
+                    for (int b = 0; b < D / 64; ++b)
+                        pk_tma3(smem + L::kQ + t * L::kTile + b * 16384, &maps.q, 64 * b, head0, q0 + j0 + t * PT,
+                                &B->q_full);
+                };
+                mbar_expect_tx(&B->q_full, n0 > 0 && n1 > 0 ? 2 * qbytes : qbytes);
+                if (n0 > 0) load_q(0);
+                auto raw = [&](int i) -> uint64_t * {
+                    return (i & 1) && (i >> 1) >= part ? &B->v_raw[((i >> 1) - part) & 3] : nullptr;
+                };
+                int issued = 0;
+                for (int i = 0; i < 2 * nb; ++i) {
+                    const int s = i % ST;
+                    if (i >= ST && !pk_wait(&B->kv_empty[s], ((i / ST) - 1) & 1, a.err, 50)) {
+                        ok = false;
                         break;
                     }
-                    // take over a CTA of the grid that has not started
-                    if (lane == 0) {
-                        mbar_expect_tx(&B->u_got, 16);
-                        asm volatile(
-                            "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], "
-                            "[%1];" ::"r"(smem_u32(&B->claim)),
-                            "r"(smem_u32(&B->u_got))
-                            : "memory");
+                    uint64_t *bar = &B->kv_full[s];
+                    if (raw(i)) {  // lands on a barrier of its own; the ring's only keeps step
+                        pk_arrive(bar);
+                        bar = raw(i);
                     }
-                    ok = __all_sync(0xffffffffu, pk_wait(&B->u_got, claims & 1, a.err, 63));
-                    ++claims;
-                    uint4 c;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(c.x), "=r"(c.y), "=r"(c.z), "=r"(c.w)
-                                 : "r"(smem_u32(&B->claim))
-                                 : "memory");
-                    uint32_t got, x;
-                    asm volatile(
-                        "{\n .reg .b128 h;\n .reg .pred p;\n .reg .b64 lo, hi;\n mov.b64 lo, {%2, %3};\n mov.b64 hi, {%4, %5};\n"
-                        " mov.b128 h, {lo, hi};\n clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
-                        " selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
-                        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}"
-                        : "=r"(got), "=r"(x)
-                        : "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    more = ok && got;
-                    work = more ? (int)x : -1;
+                    mbar_expect_tx(bar, L::kTile);
+                    const CUtensorMap *m = (i & 1) ? &maps.v : &maps.k;
+                    for (int b = 0; b < D / 64; ++b)
+                        pk_tma3(smem + L::kRing + (size_t)s * L::kTile + b * 16384, m, 64 * b, kvh,
+                                k0 + (i >> 1) * kPkKeys, bar);
+                    ++issued;
+                    if (i == 0 && n1 > 0) load_q(1);
                 }
-                __syncwarp();
-                if (lane == 0) {
-                    B->unit[u & 1].valid = valid && ok;
-                    pk_arrive(&B->u_full[u & 1]);
-                }
-                if (!valid) break;
-                // the next one when the loads of this one have all been issued: not long before it is needed
-                ok = ok && __all_sync(0xffffffffu, pk_wait(&B->u_want, u & 1, a.err, 64));
-            }
-        } else if (warp == 9) {
-            if (pk_elect()) {
-                int stage = 0, loads[2] = {0, 0}, masked = 0;
-                uint32_t phase = 1;  // of kv_empty: the first pass over the ring waits for nothing
-                struct Issued {
-                    uint64_t *bar;
-                    uint32_t parity;
-                } last[ST];
-                int issued = 0;
-                for (int u = 0; begin(u); ++u) {
-                    const View v = view(u & 1);
-                    const int kvh = B->unit[u & 1].kvh, head0 = kvh * a.G + B->unit[u & 1].chunk * a.GT;
-                    const uint32_t qbytes = (uint32_t)(PT * a.GT) * D * 2;
-                    for (int i = 0; i < 2 * v.nb && ok; ++i) {
-                        ok = pk_wait(&B->kv_empty[stage], phase, a.err, 50);
-                        if (!ok) break;
-                        uint64_t *bar = &B->kv_full[stage];
-                        uint32_t parity = phase ^ 1;
-                        if ((i & 1) && (i >> 1) >= v.part) {
-                            // lands on a barrier of its own; the ring's only keeps step
-                            pk_arrive(bar);
-                            bar = &B->v_raw[masked & 7];
-                            parity = (masked >> 3) & 1;
-                            ++masked;
-                        }
-                        mbar_expect_tx(bar, L::kTile);
-                        const CUtensorMap *m = (i & 1) ? &maps.v : &maps.k;
-                        for (int b = 0; b < D / 64; ++b)
-                            pk_tma3(smem + L::kRing + (size_t)stage * L::kTile + b * 16384, m, 64 * b, kvh,
-                                    v.k0 + (i >> 1) * kPkKeys, bar);
-                        last[stage].bar = bar;
-                        last[stage].parity = parity;
-                        if (issued < ST) ++issued;
-                        if (++stage == ST) {
-                            stage = 0;
-                            phase ^= 1;
-                        }
-                        if (i == 0)
-                            for (int t = 0; t < 2; ++t) {
-                                if ((t ? v.n1 : v.n0) == 0) continue;
-                                if (loads[t]) ok = ok && pk_wait(&B->q_empty[t], (loads[t] - 1) & 1, a.err, 49);
-                                if (!ok) break;
-                                mbar_expect_tx(&B->q_full[t], qbytes);
-                                for (int b = 0; b < D / 64; ++b)
-                                    pk_tma3(smem + L::kQ + t * L::kTile + b * 16384, &maps.q, 64 * b, head0,
-                                            v.q0 + v.j0 + t * PT, &B->q_full[t]);
-                                ++loads[t];
-                            }
+                if (!ok)  // no copy of this CTA may land after it has left
+                    for (int i = max(0, issued - ST); i < issued; ++i) {
+                        if (raw(i))
+                            pk_wait(raw(i), (((i >> 1) - part) >> 2) & 1, a.err, 51);
+                        else
+                            pk_wait(&B->kv_full[i % ST], (i / ST) & 1, a.err, 51);
                     }
-                    pk_arrive(&B->u_empty[u & 1]);
-                    pk_arrive(&B->u_want);
-                }
-                if (!ok) {  // no copy of this CTA may land after it has left
-                    for (int i = 0; i < issued; ++i) pk_wait(last[i].bar, last[i].parity, a.err, 51);
-                    for (int t = 0; t < 2; ++t)
-                        if (loads[t]) pk_wait(&B->q_full[t], (loads[t] - 1) & 1, a.err, 51);
-                }
             }
         } else if (warp == 8) {
-            if (pk_elect()) {
+            if (nb > 0 && pk_elect()) {
                 constexpr uint32_t fmt = (1u << 4) | (PkType<T>::fmt << 7) | (PkType<T>::fmt << 10) | (8u << 24);
                 constexpr uint32_t id_qk = fmt | (uint32_t)(kPkKeys >> 3) << 17;
                 constexpr uint32_t id_pv = fmt | (1u << 16) | (uint32_t)(D >> 3) << 17;  // B (V) MN-major
@@ -607,152 +501,115 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 // A wait costs 150 to 200 cycles even when its barrier is done (it queues behind
                 // the softmax warps' exponentials), so the waits for K and V come while the first
                 // tile's softmax still runs, and the commits that nobody waits for come last.
-                int stage = 0, masked = 0, loads0 = 0, loads1 = 0;
-                uint32_t phase = 0, done0 = 0, done1 = 0;  // blocks of each tile so far
+                int stage = 0;
+                uint32_t phase = 0;
                 auto next = [&]() {
                     if (++stage == ST) {
                         stage = 0;
                         phase ^= 1;
                     }
                 };
-                for (int u = 0; begin(u); ++u) {
-                    const View v = view(u & 1);
-                    if (v.nb > 0) {
-                        const int k_stage = stage;
-                        if (v.n0 > 0) ok = ok && pk_wait(&B->q_full[0], loads0++ & 1, a.err, 53);
-                        if (v.n1 > 0) ok = ok && pk_wait(&B->q_full[1], loads1++ & 1, a.err, 53);
-                        ok = ok && pk_wait(&B->kv_full[stage], phase, a.err, 52);
-                        if (ok) {
+                ok = pk_wait(&B->q_full, 0, a.err, 53) && pk_wait(&B->kv_full[0], 0, a.err, 52);
+                if (ok) {
+                    pk_fence_after();
+                    if (n0 > 0) qk(0, 0);
+                    if (n1 > 0) qk(1, 0);
+                    pk_commit(&B->kv_empty[0]);
+                }
+                next();
+#pragma unroll 1
+                for (int j = 0; j < nb && ok; ++j) {
+                    const int vs = stage;
+                    ok = pk_wait(&B->kv_full[vs], phase, a.err, 52);
+                    if (j >= part) ok = ok && pk_wait(&B->v_clean[(j - part) & 3], ((j - part) >> 2) & 1, a.err, 54);
+                    next();
+                    const int ks = stage;
+                    if (j + 1 < nb) ok = ok && pk_wait(&B->kv_full[ks], phase, a.err, 52);
+                    next();
+#pragma unroll 1
+                    for (int t = 0; t < 2; ++t) {
+                        const int nt = t ? n1 : n0;
+                        if (j < nt) {
+                            ok = ok && pk_wait(&B->p_half[t], j & 1, a.err, 55);
+                            if (!ok) break;
                             pk_fence_after();
-                            if (v.n0 > 0) qk(0, k_stage);
-                            if (v.n0 == 1) pk_commit(&B->q_empty[0]);
-                            if (v.n1 > 0) qk(1, k_stage);
-                            if (v.n1 == 1) pk_commit(&B->q_empty[1]);
-                            pk_commit(&B->kv_empty[k_stage]);
+                            pv(t, vs, 0, j);
+                            ok = pk_wait(&B->p_full[t], j & 1, a.err, 60);
+                            if (!ok) break;
+                            pk_fence_after();
+                            pv(t, vs, 1, 1);
+                            if (j + 1 == nt) pk_commit(&B->o_full[t]);
                         }
-                        next();
+                        if (j + 1 < nt) qk(t, ks);
                     }
-#pragma unroll 1
-                    for (int j = 0; j < v.nb && ok; ++j) {
-                        const int vs = stage;
-                        ok = pk_wait(&B->kv_full[vs], phase, a.err, 52);
-                        if (j >= v.part) {
-                            ok = ok && pk_wait(&B->v_clean[masked & 7], (masked >> 3) & 1, a.err, 54);
-                            ++masked;
-                        }
-                        next();
-                        const int ks = stage;
-                        if (j + 1 < v.nb) {
-                            ok = ok && pk_wait(&B->kv_full[ks], phase, a.err, 52);
-                            next();
-                        }
-#pragma unroll 1
-                        for (int t = 0; t < 2; ++t) {
-                            const int nt = t ? v.n1 : v.n0;
-                            if (j < nt) {
-                                const uint32_t par = (t ? done1++ : done0++) & 1;
-                                ok = ok && pk_wait(&B->p_half[t], par, a.err, 55);
-                                if (!ok) break;
-                                pk_fence_after();
-                                pv(t, vs, 0, j);
-                                ok = pk_wait(&B->p_full[t], par, a.err, 60);
-                                if (!ok) break;
-                                pk_fence_after();
-                                pv(t, vs, 1, 1);
-                                if (j + 1 == nt) pk_commit(&B->o_full[t]);
-                            }
-                            if (j + 1 < nt) {
-                                qk(t, ks);
-                                if (j + 2 == nt) pk_commit(&B->q_empty[t]);
-                            }
-                        }
-                        if (ok) {
-                            pk_commit(&B->kv_empty[vs]);
-                            if (j + 1 < v.nb) pk_commit(&B->kv_empty[ks]);
-                        }
+                    if (ok) {
+                        pk_commit(&B->kv_empty[vs]);
+                        if (j + 1 < nb) pk_commit(&B->kv_empty[ks]);
                     }
-                    pk_arrive(&B->u_empty[u & 1]);
                 }
             }
         } else {
             // ---- V of the blocks that are seen in part
-            int stage = 0, masked = 0;
-            for (int u = 0; __all_sync(0xffffffffu, begin(u)); ++u) {
-                const View v = view(u & 1);
-                for (int i = lane; i < D; i += 32) B->bad_key[u & 1][i] = 0x7fffffff;
-                if (lane == 0) B->bad[u & 1] = 0;
-                __syncwarp();
-                stage = (stage + 2 * min(v.part, v.nb)) % ST;
-                for (int j = v.part; j < v.nb && ok; ++j) {
-                    ok = __all_sync(0xffffffffu, pk_wait(&B->v_raw[masked & 7], (masked >> 3) & 1, a.err, 56));
-                    if (!ok) break;
-                    uint8_t *vb = smem + L::kRing + (size_t)((stage + 1) % ST) * L::kTile;
-                    const int live = min(kPkKeys, v.kl - j * kPkKeys);
-                    // 16-byte chunks: chunk c of key row r lies at place c ^ (r & 7) of its 128 bytes
-                    constexpr uint32_t e = PkType<T>::exp_one;
-                    uint4 *vq = reinterpret_cast<uint4 *>(vb) + lane;
+            const int ct = tid - 320;  // 0..63
+            for (int j = part; j < nb && ok; ++j) {
+                const int s = (2 * j + 1) % ST, c = j - part;
+                if (!pk_wait(&B->v_raw[c & 3], (c >> 2) & 1, a.err, 56)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *vb = smem + L::kRing + (size_t)s * L::kTile;
+                const int live = min(kPkKeys, kl - j * kPkKeys);
+                // 16-byte chunks: chunk c of key row r lies at place c ^ (r & 7) of its 128 bytes
+                constexpr uint32_t e = PkType<T>::exp_one;
+                uint4 *vq = reinterpret_cast<uint4 *>(vb) + ct;
 #pragma unroll 1
-                    for (int q = 0; q < kPkKeys * D / 8; q += 8 * 32) {
-                        uint4 w8[8];
-                        uint32_t hit = 0;
+                for (int q = 0; q < kPkKeys * D / 8; q += 8 * 64) {
+                    uint4 u[8];
+                    uint32_t hit = 0;
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) w8[x] = vq[q + 32 * x];
+                    for (int x = 0; x < 8; ++x) u[x] = vq[q + 64 * x];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            const int r = ((lane + q + 32 * x) >> 3) & 127;
-                            if (r >= live)
-                                vq[q + 32 * x] = make_uint4(0, 0, 0, 0);
-                            else
-                                hit |= ((w8[x].x & 0x7fff7fffu) + e) | ((w8[x].y & 0x7fff7fffu) + e) |
-                                       ((w8[x].z & 0x7fff7fffu) + e) | ((w8[x].w & 0x7fff7fffu) + e);
-                        }
-                        if (hit & 0x80008000u) {  // rare
-                            unsigned short *h = reinterpret_cast<unsigned short *>(vq + q);
+                    for (int x = 0; x < 8; ++x) {
+                        const int r = ((ct + q + 64 * x) >> 3) & 127;
+                        if (r >= live)
+                            vq[q + 64 * x] = make_uint4(0, 0, 0, 0);
+                        else
+                            hit |= ((u[x].x & 0x7fff7fffu) + e) | ((u[x].y & 0x7fff7fffu) + e) |
+                                   ((u[x].z & 0x7fff7fffu) + e) | ((u[x].w & 0x7fff7fffu) + e);
+                    }
+                    if (hit & 0x80008000u) {  // rare
+                        unsigned short *v = reinterpret_cast<unsigned short *>(vq + q);
 #pragma unroll 1
-                            for (int y = 0; y < 64; ++y) {
-                                const int x = y >> 3, c = lane + q + 32 * x, r = (c >> 3) & 127;
-                                unsigned short *w = h + 32 * 8 * x + (y & 7);
-                                if (r < live && ((*w & 0x7fffu) + (e & 0xffffu)) & 0x8000u) {
-                                    *w = 0;
-                                    atomicMin(&B->bad_key[u & 1][(c >> 10) * 64 + ((c & 7) ^ (r & 7)) * 8 + (y & 7)],
-                                              j * kPkKeys + r);
-                                    B->bad[u & 1] = 1;
-                                }
+                        for (int y = 0; y < 64; ++y) {
+                            const int x = y >> 3, c = ct + q + 64 * x, r = (c >> 3) & 127;
+                            unsigned short *w = v + 64 * 8 * x + (y & 7);
+                            if (r < live && ((*w & 0x7fffu) + (e & 0xffffu)) & 0x8000u) {
+                                *w = 0;
+                                atomicMin(&B->bad_key[(c >> 10) * 64 + ((c & 7) ^ (r & 7)) * 8 + (y & 7)],
+                                          j * kPkKeys + r);
+                                B->bad = 1;
                             }
                         }
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    pk_arrive(&B->v_clean[masked & 7]);
-                    ++masked;
-                    stage = (stage + 2) % ST;
                 }
-                __syncwarp();
-                if (lane == 0) pk_arrive(&B->u_empty[u & 1]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                pk_arrive(&B->v_clean[c & 3]);
             }
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        // ---- softmax: thread = row of tile t
-        const int t = warp >> 2, row = tid & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const uint32_t s_t = tmem + t * 128 + lanes, o_t = tmem + 256 + t * 128 + lanes;
-        uint32_t done = 0, ends = 0;  // blocks, and units with blocks, so far
-        int masked = 0;
-        bool joined = false;  // a cluster's barriers: every CTA passes each once, whatever its unit
-        for (int u = 0; __all_sync(0xffffffffu, begin(u)); ++u) {
-            int nt, lim, lim0, seen_last;  // seen_last: the clearing of the tile's last block (-1: none)
-            {
-                const View v = view(u & 1);
-                nt = t ? v.n1 : v.n0;
-                lim = v.shift + v.j0 + t * PT + row / a.GT;  // last key that this row sees
-                lim0 = v.shift + v.j0 + t * PT;              // of the tile's first row
-                seen_last = nt > v.part ? masked + nt - 1 - v.part : -1;
-                masked += max(0, v.nb - v.part);
-            }
+        } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+            // ---- softmax: thread = row of tile t
+            const int t = warp >> 2, row = tid & 127;
+            const int nt = t ? n1 : n0;
+            const int jq = j0 + t * PT + row / a.GT;  // query of this row
+            const int lim = shift + jq;               // last key that it sees
+            const int lim0 = shift + j0 + t * PT;     // of the tile's first row
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+            const uint32_t s_t = tmem + t * 128 + lanes, o_t = tmem + 256 + t * 128 + lanes;
             float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to
             for (int j = 0; j < nt; ++j) {
                 // (the warp leaves as one: what follows is warp-wide)
-                if (!__all_sync(0xffffffffu, pk_wait(&B->s_full[t], done++ & 1, a.err, 57))) {
+                if (!__all_sync(0xffffffffu, pk_wait(&B->s_full[t], j & 1, a.err, 57))) {
                     ok = false;
                     break;
                 }
@@ -764,8 +621,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 if (j * kPkKeys + kPkKeys - 1 > lim0) {
                     const int seen = lim - j * kPkKeys;  // keys of the block up to this one
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i > seen) sv[i] = 0xff800000u;
+                    for (int w = 0; w < 4; ++w) {
+                        const int s = seen - 32 * w;
+                        const uint32_t bits = s >= 31 ? 0xffffffffu : s < 0 ? 0u : (2u << s) - 1u;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!(bits >> i & 1u)) sv[32 * w + i] = 0xff800000u;
+                    }
                 }
                 // exponentials of keys 64 c .. 64 c + 63, their sum and P; FIND: the maximum of the
                 // block's 128 scores on the way (it uses another pipe than the exponentials)
@@ -793,16 +655,14 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
                 };
                 // The first half is computed with the maximum so far while this block's is
-                // found, and again in the rare case that the maximum moves (the first block's
-                // is found beforehand).
+                // found, and again in the rare case that the maximum moves.  (Before the first
+                // block, the maximum of 16 keys is near enough: code that runs once per unit
+                // costs its way through the instruction cache.)
                 f32x2 sum[2];
                 uint32_t pv[32];
                 if (j == 0) {
-                    float x = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2)
-                        x = fmaxf(x, fmaxf(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])));
-                    m = x;
+                    for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(sv[i]));
                 }
                 half(0, true, m, sum, pv);
                 const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
@@ -839,14 +699,11 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 }
             }
             // ---- epilogue
-            if (nt > 0 && ok && !__all_sync(0xffffffffu, pk_wait(&B->o_full[t], ends++ & 1, a.err, 58))) ok = false;
+            if (nt > 0 && ok && !__all_sync(0xffffffffu, pk_wait(&B->o_full[t], 0, a.err, 58))) ok = false;
             pk_fence_after();
-            // what the clearing warp noted of this tile's blocks
-            bool bad = false;
-            if (seen_last >= 0 && ok) {
-                pk_wait(&B->v_clean[seen_last & 7], (seen_last >> 3) & 1, a.err, 59);
-                bad = B->bad[u & 1];
-            }
+            // what the clearing warps noted of this tile's blocks
+            if (nt > part && ok) pk_wait(&B->v_clean[(nt - 1 - part) & 3], ((nt - 1 - part) >> 2) & 1, a.err, 59);
+            const bool bad = nt > 0 && B->bad;
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees nothing has O = 0 and l = 0
             // 32 values of this row from TMEM
             auto load_o = [&](int c, uint32_t(&ov)[32]) {
@@ -858,61 +715,64 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     for (int i = 0; i < 32; ++i) ov[i] = 0;
                 }
                 if (bad) {
+                    const int4 *key = reinterpret_cast<const int4 *>(&B->bad_key[32 * c]);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (B->bad_key[u & 1][32 * c + i] <= lim) ov[i] = 0x7fc00000u;
+                    for (int i = 0; i < 8; ++i) {
+                        const int4 k = key[i];
+                        ov[4 * i] = k.x <= lim ? 0x7fc00000u : ov[4 * i];
+                        ov[4 * i + 1] = k.y <= lim ? 0x7fc00000u : ov[4 * i + 1];
+                        ov[4 * i + 2] = k.z <= lim ? 0x7fc00000u : ov[4 * i + 2];
+                        ov[4 * i + 3] = k.w <= lim ? 0x7fc00000u : ov[4 * i + 3];
+                    }
                 }
             };
-            // where row x of tile s goes (null: nowhere)
+            // Where row x of tile s goes (null: nowhere).  (The unit is read again from shared
+            // memory, which keeps the loop over the blocks free of what only the end needs.)
             auto row_out = [&](int s, int x) -> T * {
-                const PkUnit &un = B->unit[u & 1];
-                const int j = un.j0 + s * PT + x / a.GT, h = un.chunk * a.GT + x % a.GT;
-                if (x >= PT * a.GT || j >= un.ql || h >= a.G || !ok) return nullptr;
-                return reinterpret_cast<T *>(a.out) + (long)(un.q0 + j) * a.out_rs + (long)(un.kvh * a.G + h) * D;
+                const int j = B->found[1] * 2 * PT + s * PT + x / a.GT, h = chunk * a.GT + x % a.GT;
+                if (x >= PT * a.GT || j >= B->found[3] || h >= a.G || !ok) return nullptr;
+                return reinterpret_cast<T *>(a.out) + (long)(B->found[2] + j) * a.out_rs + (long)(kvh * a.G + h) * D;
             };
             if (a.split == 1) {
-                // the warp's 32 rows, 64 dimensions at a time, through shared memory, so that a row is
-                // written by consecutive lanes; 16-byte chunk c of row r at place c ^ (r & 7)
-                uint4 *buf = reinterpret_cast<uint4 *>(smem + L::kOut) + warp * 256;
+                // The warp's rows through the part of the Q tile that they came from (all products
+                // that read it are complete), so that a row is written by consecutive lanes.
+                constexpr int C = D / 8;  // 16-byte chunks per row, chunk c of row r at place c ^ (r & 7)
+                uint4 *buf = reinterpret_cast<uint4 *>(smem + L::kQ + t * L::kTile) + (warp & 3) * 32 * C;
                 const T *own = row_out(t, row);  // the row in this lane's registers
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t ov[32], w[16];
+                    load_o(c, ov);
 #pragma unroll
-                for (int p = 0; p < D / 64; ++p) {
+                    for (int i = 0; i < 16; ++i)
+                        w[i] = PkType<T>::pack(__uint_as_float(ov[2 * i]) * inv, __uint_as_float(ov[2 * i + 1]) * inv);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t ov[32], w[16];
-                        load_o(2 * p + c, ov);
+                    for (int i = 0; i < 4; ++i)
+                        buf[lane * C + ((4 * c + i) ^ (lane & 7))] =
+                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+                __syncwarp();
+                const int c = lane % C;  // this lane's chunk of each row that it writes
+#pragma unroll 2
+                for (int x = 0; x < C; ++x) {
+                    const int r = x * (32 / C) + lane / C;
+                    T *o = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, (unsigned long long)own, r));
+                    const uint4 v = buf[r * C + (c ^ (r & 7))];
+                    if (o && a.vec) {
+                        reinterpret_cast<uint4 *>(o)[c] = v;
+                    } else if (o) {
+                        unsigned short *e = reinterpret_cast<unsigned short *>(o) + 8 * c;
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            w[i] = PkType<T>::pack(__uint_as_float(ov[2 * i]) * inv, __uint_as_float(ov[2 * i + 1]) * inv);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            buf[lane * 8 + ((4 * c + i) ^ (lane & 7))] =
-                                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                    }
-                    __syncwarp();
-                    const int c = lane % 8;  // this lane's chunk of each row that it writes
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const int r = x * 4 + lane / 8;
-                        T *o = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, (unsigned long long)own, r));
-                        const uint4 v = buf[r * 8 + (c ^ (r & 7))];
-                        if (o && a.vec) {
-                            reinterpret_cast<uint4 *>(o + 64 * p)[c] = v;
-                        } else if (o) {
-                            unsigned short *e = reinterpret_cast<unsigned short *>(o + 64 * p) + 8 * c;
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                e[2 * i] = (unsigned short)w[i];
-                                e[2 * i + 1] = (unsigned short)(w[i] >> 16);
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            e[2 * i] = (unsigned short)w[i];
+                            e[2 * i + 1] = (unsigned short)(w[i] >> 16);
                         }
                     }
-                    __syncwarp();
                 }
             } else {
                 // O as it stands into the ring, which the products of both tiles have left (16-byte
-                // chunk c of row r at place c ^ (r & 7)), the maxima and sums beside it
+                // chunk c of row r at place c ^ (r & 7)), the maxima and sums into the Q tiles' place
                 constexpr int C = D / 4;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 float4 *buf = reinterpret_cast<float4 *>(smem + L::kRing) + (t * 128 + row) * C;
@@ -926,7 +786,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                             make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]),
                                         __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
                 }
-                float *part_m = reinterpret_cast<float *>(smem + L::kOut), *part_l = part_m + 256;
+                float *part_m = reinterpret_cast<float *>(smem + L::kQ), *part_l = part_m + 256;
                 part_m[tid] = m * a.scale_log2;
                 part_l[tid] = l;
                 pk_cluster_sync();
@@ -963,24 +823,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         e[3] = (unsigned short)(w1 >> 16);
                     }
                 }
-                pk_cluster_sync();  // no CTA leaves while its part is read
-                joined = true;
             }
-            pk_fence_before();
+        }
+        if (a.split > 1) {
             __syncwarp();
-            if (lane == 0) pk_arrive(&B->u_empty[u & 1]);
+            if (warp >= 8) pk_cluster_sync();  // the softmax warps' first
+            pk_cluster_sync();                 // no CTA leaves while its part is read
         }
-        __syncwarp();
-        if (a.split > 1 && !joined) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            pk_cluster_sync();
-            pk_cluster_sync();
-        }
-    }
-    __syncwarp();
-    if (a.split > 1 && warp >= 8) {  // with the softmax warps' two
-        pk_cluster_sync();
-        pk_cluster_sync();
     }
     pk_fence_before();
     __syncthreads();
