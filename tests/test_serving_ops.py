@@ -679,3 +679,253 @@ def test_packed_later_keys_do_not_touch_earlier_queries(dev, bad, hd):
             assert (np.abs(got - want) <= tol)[~seen].all()
         elif np.isnan(bad):
             assert np.isnan(got[137:, : 2 * hd]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [wk.F16, wk.BF16])
+def test_packed_many_short_sequences_and_a_late_start(dev, dt):
+    """More sequences than one pass over their lengths takes; the first starts behind rows of nobody."""
+    rng = np.random.default_rng(5)
+    ql = rng.integers(0, 4, 900)
+    kl = ql + rng.integers(0, 3, 900)
+    c = make_packed([7, *ql], [9, *kl], 6, 3, 64, dt, seed=17)
+    want, tol = ref_packed(c)
+    d = dict(c, qs=c["qs"][1:], ks=c["ks"][1:])
+    got = run_packed(dev, d)
+    assert (to_bits(got[:7], dt).view(np.uint16) == 0x3555).all()  # not written
+    close(got[7:], want[7:], tol[7:])
+    assert np.array_equal(got[7:], run_packed(dev, d)[7:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [0, 1])
+def test_packed_without_keys(dev, shift):
+    c = make_packed([5, 70], [0, 0], 4, 2, 64, wk.F16, seed=1)
+    assert not run_packed(dev, c, shift=shift, tail=0).any()
+
+
+# ------------------------------------------------------------------ other ways to share the work out
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,heads,kv,hd,dt", [
+    (list(range(3, 2400, 57)), 8, 2, 64, wk.F16),            # equal runs, parts joined by the last to arrive
+    ([0, 1800, -1, 900, 33, 0, 1200, 64] * 4, 32, 8, 128, wk.BF16),
+    ([4000, 1, 30, 70] * 5, 32, 2, 128, wk.F16),             # 16 heads per K/V head; long rows among short ones
+    ([150000], 4, 1, 64, wk.F16),                            # one row: a second launch joins the parts
+    ([70000, 0, 70000], 40, 2, 128, wk.BF16),
+    ([5] * 2100, 2, 1, 64, wk.F16),                          # more rows than equal runs take
+])
+def test_decode_shares(dev, lens, heads, kv, hd, dt):
+    c = make_decode([n - 1 for n in lens], heads, kv, hd, dt, seed=len(lens) + hd)
+    want, tol = ref_decode(c)
+    got = run_decode(dev, c, max(lens), ws=True)
+    close(got, want, tol)
+    assert np.array_equal(got, run_decode(dev, c, max(lens), ws=True))
+    close(run_decode(dev, c, max(lens), ws=False), want, tol)
+
+
+@pytest.mark.gpu
+def test_decode_workspace_serves_calls_of_other_sizes(dev):
+    """One workspace through calls of different shapes, in turn, each as from a fresh one."""
+    cases = [make_decode([n - 1 for n in lens], *shape, seed=7) for lens, shape in (
+        (list(range(3, 2400, 57)), (8, 2, 64, wk.F16)), ([150000], (4, 1, 64, wk.F16)),
+        ([4000, 1, 30, 70] * 5, (32, 2, 128, wk.F16)))]
+    n = max(dev.wk_kv8_attention_ws(len(c["pos"]), int(c["pos"].max()) + 1, c["heads"], c["kv"], c["hd"]) for c in cases)
+    ws = up(np.zeros(n, np.uint8))
+    for c in [*cases, *cases[::-1]]:
+        want, tol = ref_decode(c)
+        rows, w = c["q"].shape
+        b = [up(v) for v in (np.zeros((rows, w), np.float16), to_bits(c["q"], c["dt"]), *c["codes"],
+                             *(s.astype(np.float32) for s in c["scales"]), c["table"].astype(np.int32),
+                             c["seq"].astype(np.int32), c["pos"].astype(np.int32))]
+        wk.check(dev.wk_kv8_attention(b[0], w, b[1], w, b[2], b[3], b[4], b[5], c["n_pages"], b[6], *c["table"].shape,
+                                      b[7], b[8], rows, int(c["pos"].max()) + 1, c["heads"], c["kv"], c["hd"], c["dt"],
+                                      ws, n))
+        close(down(b[0], (rows, w), np.float16).astype(np.float64), want, tol)
+        free(*b)
+    free(ws)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(dev):
+    """A cache of more than 2^32 bytes: stored to and read from pages at both ends."""
+    kv, hd = 8, 128
+    page_bytes = kv * PAGE * hd
+    n_pages = (1 << 32) // page_bytes + 40
+    pools = [alloc(n_pages * page_bytes) for _ in range(2)]
+    scales = [up(np.ones((n_pages, kv), np.float32)) for _ in range(2)]
+    rng = np.random.default_rng(3)
+    lens = np.array([150, 70])
+    table = np.array([[n_pages - 1, 0, n_pages - 3], [n_pages - 2, 1, -1]])
+    starts = np.array([0, 150, 220])
+    x = [rounded(rng.standard_normal((220, kv * hd)), wk.F16) for _ in range(2)]
+    b = [up(to_bits(v, wk.F16)) for v in x] + [up(v.astype(np.int32)) for v in (starts, np.zeros(2), table)]
+    wk.check(dev.wk_kv8_store(*pools, *scales, n_pages, b[0], kv * hd, b[1], kv * hd, b[2], b[3], 2, 220, b[4], 3, kv, hd,
+                              wk.F16))
+    c = dict(pos=lens - 1, seq=np.arange(2), table=np.where(table < 0, -1, np.searchsorted([0, 1, n_pages - 3, n_pages - 2,
+             n_pages - 1], table)), heads=16, kv=kv, hd=hd, dt=wk.F16, n_pages=5,
+             q=rounded(rng.standard_normal((2, 16 * hd)), wk.F16))
+    codes, sc = zip(*(ref_store(np.zeros((5, kv, PAGE, hd), np.uint8), np.ones((5, kv)), v.reshape(220, kv, hd), starts,
+                                [0, 0], c["table"], 5) for v in x))
+    want, tol = ref_decode(dict(c, codes=list(codes), scales=list(sc)))
+    q, out, seq, pos = up(to_bits(c["q"], wk.F16)), alloc(2 * c["q"].size), up(np.arange(2, dtype=np.int32)), \
+        up((lens - 1).astype(np.int32))
+    wk.check(dev.wk_kv8_attention(out, 16 * hd, q, 16 * hd, *pools, *scales, n_pages, b[4], 2, 3, seq, pos, 2, 150, 16, kv,
+                                  hd, wk.F16, None, 0))
+    close(down(out, c["q"].shape, np.float16).astype(np.float64), want, tol)
+    free(*pools, *scales, *b, q, out, seq, pos)
+
+
+@pytest.mark.gpu
+def test_packed_rows_beyond_32_bits(dev):
+    """Rows so far apart that the last ones lie more than 2^32 bytes behind the first."""
+    c = make_packed([30, 9], [30, 40], 2, 1, 64, wk.F16, seed=3)
+    rs = 1 << 26  # elements: 128 MB from row to row
+    q, k, v, out = (alloc(2 * (n - 1) * rs + 2 * w) for n, w in ((39, 128), (70, 64), (70, 64), (39, 128)))
+    L = wk.lib()
+    for p, x in ((q, c["q"]), (k, c["k"]), (v, c["v"])):
+        bits = to_bits(x, wk.F16)
+        for r in range(len(x)):
+            L.cuda_to_device(p + 2 * r * rs, as_p(np.ascontiguousarray(bits[r])), bits[r].nbytes)
+    qs, ks = up(c["qs"].astype(np.int32)), up(c["ks"].astype(np.int32))
+    wk.check(L.wk_attention_packed(out, rs, q, rs, k, rs, v, rs, qs, ks, 2, 39, 70, 2, 1, 64, wk.F16))
+    got = np.stack([down(out + 2 * r * rs, 128, np.float16) for r in range(39)]).astype(np.float64)
+    want, tol = ref_packed(c)
+    close(got, want, tol)
+    free(q, k, v, out, qs, ks)
+
+
+# ------------------------------------------------------------------ a serving loop
+
+class Loop:
+    """Sequences of one layer over the four entry points, and what the cache should hold, in 64 bits."""
+
+    def __init__(self, dev, n, heads, kv, hd, dt, n_pages, max_pages, rows_cap, seed):
+        self.dev, self.n, self.heads, self.kv, self.hd, self.dt = dev, n, heads, kv, hd, dt
+        self.n_pages, self.max_pages, self.rows_cap = n_pages, max_pages, rows_cap
+        self.rng = np.random.default_rng(seed)
+        self.w = (heads + 2 * kv) * hd
+        self.ws_bytes = dev.wk_kv8_attention_ws(rows_cap, max_pages * PAGE, heads, kv, hd)
+        i32 = lambda *s: up(np.zeros(s, np.int32))  # noqa: E731
+        self.free_list = self.rng.permutation(n_pages)
+        self.taken = 0
+        self.d = dict(k=up(np.zeros(n_pages * kv * PAGE * hd, np.uint8)), v=up(np.zeros(n_pages * kv * PAGE * hd, np.uint8)),
+                      ks=up(np.ones((n_pages, kv), np.float32)), vs=up(np.ones((n_pages, kv), np.float32)),
+                      table=up(np.full((n, max_pages), -1, np.int32)), starts=i32(n + 1), ctx=i32(n), lens=i32(n),
+                      seq=i32(rows_cap), pos=i32(rows_cap), slot=up(np.zeros(rows_cap, np.int64)), status=i32(3),
+                      add=i32(n), free=up(self.free_list.astype(np.int32)), n_free=up(np.array([n_pages], np.int32)),
+                      qkv=up(np.zeros((rows_cap, self.w), np.uint16)), out=up(np.zeros((rows_cap, heads * hd), np.uint16)),
+                      ws=up(np.zeros(max(self.ws_bytes, 16), np.uint8)))
+        self.ctx = np.zeros(n, int)
+        self.table = np.full((n, max_pages), -1)
+        self.codes = [np.zeros((n_pages, kv, PAGE, hd), np.uint8) for _ in range(2)]
+        self.scales = [np.ones((n_pages, kv)) for _ in range(2)]
+
+    def put(self, name, x):
+        x = np.ascontiguousarray(x)
+        self.dev.cuda_to_device(self.d[name], as_p(x), x.nbytes)
+
+    def inputs(self, add):
+        """New rows of the sequences, the lengths and the rest of the free list."""
+        self.add = np.array(add)
+        rows = int(self.add.sum())
+        self.x = rounded(self.rng.standard_normal((rows, self.w)) * self.rng.choice([0.5, 1.0, 3.0], (rows, 1)), self.dt)
+        self.put("qkv", to_bits(self.x, self.dt))
+        self.put("ctx", self.ctx.astype(np.int32))
+        self.put("add", self.add.astype(np.int32))
+        self.put("free", np.roll(self.free_list, -self.taken).astype(np.int32))
+        self.put("n_free", np.array([self.n_pages - self.taken], np.int32))
+
+    def launch(self, prompts):
+        """One step: its calls, and nothing that waits."""
+        D, d, es = self.dev, self.d, 2
+        wk.check(D.wk_batch_plan(d["starts"], d["lens"], d["seq"], d["pos"], d["slot"], self.rows_cap, d["table"],
+                                 self.max_pages, d["status"], d["ctx"], d["add"], self.n, d["free"], d["n_free"],
+                                 self.n_pages))
+        q, k, v = d["qkv"], d["qkv"] + es * self.heads * self.hd, d["qkv"] + es * (self.heads + self.kv) * self.hd
+        wk.check(D.wk_kv8_store(d["k"], d["v"], d["ks"], d["vs"], self.n_pages, k, self.w, v, self.w, d["starts"], d["ctx"],
+                                self.n, self.rows_cap, d["table"], self.max_pages, self.kv, self.hd, self.dt))
+        ow = self.heads * self.hd
+        if prompts:
+            wk.check(D.wk_attention_packed(d["out"], ow, q, self.w, k, self.w, v, self.w, d["starts"], d["starts"], self.n,
+                                           self.rows_cap, self.rows_cap, self.heads, self.kv, self.hd, self.dt))
+        else:
+            wk.check(D.wk_kv8_attention(d["out"], ow, q, self.w, d["k"], d["v"], d["ks"], d["vs"], self.n_pages,
+                                        d["table"], self.n, self.max_pages, d["seq"], d["pos"], self.rows_cap,
+                                        self.max_pages * PAGE, self.heads, self.kv, self.hd, self.dt, d["ws"],
+                                        self.ws_bytes))
+
+    def verify(self, prompts):
+        p = ref_plan(self.ctx, self.add, self.table, np.roll(self.free_list, -self.taken), self.n_pages - self.taken,
+                     self.rows_cap)
+        for name, key, t in (("seq", "row_seq", np.int32), ("pos", "row_pos", np.int32), ("slot", "row_slot", np.int64),
+                             ("table", "table", np.int32), ("lens", "lens", np.int32), ("status", "status", np.int32)):
+            assert np.array_equal(down(self.d[name], p[key].shape, t), p[key]), name
+        self.table = p["table"]
+        rows, H, kv, hd = len(self.x), self.heads * self.hd, self.kv, self.hd
+        for i, name in enumerate("kv"):
+            x = self.x[:, H + i * kv * hd:H + (i + 1) * kv * hd].reshape(rows, kv, hd)
+            self.codes[i], self.scales[i] = ref_store(self.codes[i], self.scales[i], x, p["starts"], self.ctx, self.table,
+                                                      self.n_pages)
+            got = down(self.d[name], self.codes[i].shape, np.uint8)
+            assert same_codes(got, self.codes[i]).all()
+            assert np.array_equal(down(self.d[name + "s"], (self.n_pages, kv), np.float32), self.scales[i])
+        out = from_bits(down(self.d["out"], (self.rows_cap, H), RAW[self.dt]), self.dt)
+        c = dict(heads=self.heads, kv=kv, hd=hd, dt=self.dt, q=self.x[:, :H])
+        if prompts:
+            want, tol = ref_packed(dict(c, k=self.x[:, H:H + kv * hd], v=self.x[:, H + kv * hd:], qs=p["starts"],
+                                        ks=p["starts"]))
+        else:
+            want, tol = ref_decode(dict(c, pos=p["row_pos"][:rows], seq=p["row_seq"][:rows], table=self.table,
+                                        codes=self.codes, scales=self.scales, n_pages=self.n_pages))
+            assert not out[rows:].any()  # the rows behind the last sequence have no position: zeros
+        close(out[:rows], want, tol)
+        self.taken += int(p["status"][1])
+        self.ctx = p["lens"]
+
+    def end(self):
+        free(*self.d.values())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,dt", [(8, 2, 64, wk.F16), (8, 1, 128, wk.BF16)])
+def test_serving_loop(dev, heads, kv, hd, dt):
+    """Prompts, then steps in which sequences bring one token, several, or none; pages are taken as they fill."""
+    loop = Loop(dev, 5, heads, kv, hd, dt, n_pages=40, max_pages=8, rows_cap=400, seed=hd)
+    adds = [[64, 130, 1, 63, 0], [1, 1, 1, 1, 0], [1, 0, 1, 1, 0], [3, 1, 62, 1, 90], [1, 1, 1, 1, 1]]
+    for i, add in enumerate(adds):
+        loop.inputs(add)
+        loop.launch(prompts=i == 0)
+        loop.verify(prompts=i == 0)
+    loop.end()
+
+
+@pytest.mark.gpu
+def test_serving_loops_captured_and_replayed_in_turn(dev):
+    """Two loops' steps as graphs that run in turn, each with a workspace of its own, beside calls made directly."""
+    torch = pytest.importorskip("torch")
+    stream = torch.cuda.ExternalStream(dev.wk_stream())
+    loops = [Loop(dev, 6, 8, 2, 128, wk.F16, 60, 8, 128, seed=1), Loop(dev, 3, 4, 4, 64, wk.BF16, 40, 16, 96, seed=2)]
+    graphs = []
+    for loop, prompt in zip(loops, ([20, 30, 1, 0, 5, 64], [90, 1, 3])):
+        loop.inputs(prompt)
+        loop.launch(prompts=True)
+        loop.verify(prompts=True)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            loop.launch(prompts=False)
+        graphs.append(g)
+    for step in range(4):
+        for loop, g in zip(loops, graphs):
+            loop.inputs([1] * loop.n if step % 2 == 0 else [int(i != step % loop.n) for i in range(loop.n)])
+            with torch.cuda.stream(stream):
+                g.replay()
+            loop.verify(prompts=False)
+        loops[0].inputs([2] * loops[0].n)
+        loops[0].launch(prompts=False)
+        loops[0].verify(prompts=False)
+    torch.cuda.synchronize()
+    del graphs, g
+    for loop in loops:
+        loop.end()
