@@ -250,14 +250,25 @@ struct Kv8Attn {
 #endif
 constexpr int kSegCost = WK_SEGCOST;
 constexpr int kTickets = 4096;  // at most so many CTAs
-// the run that has place x of the cost
-__device__ __forceinline__ int kv8_owner(long long x, long long runs, long long total) {
-    return (int)(((x + 1) * runs - 1) / total);
-}
-__device__ __forceinline__ long long kv8_runs(long long total, int ctas) {
-    const long long most = (total + kSegCost + 7) / (kSegCost + 8);
-    return most < ctas ? (most > 0 ? most : 1) : ctas;
-}
+struct Kv8Runs {
+    int total, runs, q, r;
+    __device__ __forceinline__ Kv8Runs(int total_, int ctas) : total(total_) {
+        const int most = (total + kSegCost + 7) / (kSegCost + 8);
+        runs = max(1, min(most, ctas));
+        q = total / runs;
+        r = total % runs;
+    }
+    // c total / runs, without a 64-bit division (several of those took 0.7 us of a launch)
+    __device__ __forceinline__ int begin(int c) const { return c * q + c * r / runs; }
+    // the run that has place x of the cost
+    __device__ __forceinline__ int owner(int x) const {
+        int c = (int)((float)x * (float)runs / (float)total);
+        c = max(0, min(c, runs - 1));
+        while (c > 0 && begin(c) > x) --c;
+        while (c + 1 < runs && begin(c + 1) <= x) ++c;
+        return c;
+    }
+};
 
 __device__ __forceinline__ uint4 ldg_stream16(const void *p) {
     uint4 v;
@@ -313,9 +324,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
     constexpr int MT = D / 16;       // 16-dim tiles of O
     constexpr int VW = D / 32;       // 32-bit words of a V row per lane
     constexpr int kPart = D + 4;     // floats of a part: O, m, l, 2 unused
-    __shared__ float s_o[kAtWarps][HB][D];
+    __shared__ __align__(16) float s_o[kAtWarps][HB][D];
     __shared__ float s_m[kAtWarps][HB], s_l[kAtWarps][HB];
-    __shared__ float s_co[kEven ? 1 : HB][D], s_cm[HB], s_cl[HB];  // this CTA's part, read by the cluster
+    __shared__ __align__(16) float s_co[kEven ? 1 : HB][D];
+    __shared__ float s_cm[HB], s_cl[HB];  // this CTA's part, read by the cluster
     extern __shared__ int s_prefix[];                              // even shares: [rows + 1]
     __shared__ int s_scan[kAtWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -330,8 +342,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
     int row, rank = 0, hc;
     int u0, u1, step;         // this warp's steps of the segment: u0, u0 + step, ... below u1
     int seg0 = 0;              // even shares: where the run stands in the head group's cost
-    long long left_cost = 0;   // even shares: what is left of this CTA's run
-    long long total = 0, runs = 0;
+    int left_cost = 0;         // even shares: what is left of this CTA's run
+    Kv8Runs runs(1, 1);
     if (kEven) {
         // cost of the rows before each
         int base = 0;
@@ -365,22 +377,21 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
             if (s_prefix[r] == s_prefix[r + 1])
                 for (int x = tid; x < a.heads * D; x += kAtWarps * 32)
                     reinterpret_cast<T *>(a.out)[(long)r * a.out_rs + x] = from_float<T>(0.f);
-        total = (long long)base * HC;
-        runs = kv8_runs(total, a.ctas);
-        if (total == 0 || blockIdx.x >= runs) return;
-        const long long b0 = blockIdx.x * total / runs;
-        left_cost = (blockIdx.x + 1) * total / runs - b0;
+        runs = Kv8Runs(base * HC, a.ctas);
+        if (base == 0 || blockIdx.x >= runs.runs) return;
+        const int b0 = runs.begin(blockIdx.x);
+        left_cost = runs.begin(blockIdx.x + 1) - b0;
         int lo = 0, hi = a.rows;  // the last row that starts at or before b0
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if ((long long)s_prefix[mid] * HC <= b0)
+            if (s_prefix[mid] * HC <= b0)
                 lo = mid;
             else
                 hi = mid;
         }
         row = lo;
         const int n = s_prefix[row + 1] - s_prefix[row];
-        const int rem = (int)(b0 - (long long)s_prefix[row] * HC);
+        const int rem = b0 - s_prefix[row] * HC;
         hc = rem / n;
         seg0 = rem % n;
     } else {
@@ -393,7 +404,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
     const long len = keys_of(row);
     const int *table = a.table + (long)(len > 0 ? a.seq[row] : 0) * a.max_pages;
     const int units = (int)((len + kAtKeys - 1) / kAtKeys);
-    const int cut = (int)min((long long)units + kSegCost, seg0 + left_cost);  // even shares: where the run leaves it
+    const int cut = min(units + kSegCost, seg0 + left_cost);  // even shares: where the run leaves it
     const int first = max(seg0 - kSegCost, 0);
     if (kEven) {
         u0 = first + warp;
@@ -671,39 +682,45 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
     const int nh = kEven && u1 <= first ? 0 : min(HB, a.G - h0);  // 0: the run ends before the first step
     const bool whole = !kEven || (first == 0 && u1 == units);
     float *part = kEven ? a.part + ((long)blockIdx.x * 2 + (first == 0)) * HB * kPart : nullptr;
-    auto put = [&](int h, int d, float m, float l, float v) {
-        if (whole) {
-            reinterpret_cast<T *>(a.out)[(long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d] =
-                from_float<T>(l > 0.f || l != l ? v / l : 0.f);
-        } else {
-            float *p = part + h * kPart;
-            p[d] = v;
-            if (d == 0) {
-                p[D] = m;
-                p[D + 1] = l;
-            }
-        }
-    };
-    for (int x = tid; x < nh * D; x += kAtWarps * 32) {
-        const int h = x / D, d = x % D;
-        float m = s_m[0][h];
+    // the warps' parts relative to the largest maximum
+    __shared__ float s_f[kAtWarps][HB];
+    if (tid < HB) {
+        float m = s_m[0][tid], l = 0.f;
 #pragma unroll
-        for (int w = 1; w < kAtWarps; ++w) m = fmaxf(m, s_m[w][h]);
-        float l = 0.f, v = 0.f;
+        for (int w = 1; w < kAtWarps; ++w) m = fmaxf(m, s_m[w][tid]);
 #pragma unroll
         for (int w = 0; w < kAtWarps; ++w) {
-            const float f = s_m[w][h] == -INFINITY ? (s_l[w][h] != s_l[w][h] ? 1.f : 0.f) : ex2(s_m[w][h] - m);
-            l += s_l[w][h] * f;
-            v += s_o[w][h][d] * f;
+            const float mw = s_m[w][tid], lw = s_l[w][tid];
+            const float f = mw == -INFINITY ? (lw != lw ? 1.f : 0.f) : ex2(mw - m);
+            s_f[w][tid] = f;
+            l += lw * f;
         }
-        if (kEven || a.cluster == 1) {
-            put(h, d, m, l, v);
+        s_cm[tid] = m;
+        s_cl[tid] = l;
+    }
+    __syncthreads();
+    for (int x = tid; x < nh * (D / 4); x += kAtWarps * 32) {
+        const int h = x / (D / 4), d = x % (D / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kAtWarps; ++w) {
+            const float f = s_f[w][h];
+            const float4 o4 = *reinterpret_cast<const float4 *>(&s_o[w][h][d]);
+            v.x += o4.x * f, v.y += o4.y * f, v.z += o4.z * f, v.w += o4.w * f;
+        }
+        if (!kEven && a.cluster > 1) {
+            *reinterpret_cast<float4 *>(&s_co[kEven ? 0 : h][d]) = v;
+        } else if (whole) {
+            const float l = s_cl[h], inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            T *dst = reinterpret_cast<T *>(a.out) + (long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d;
+            dst[0] = from_float<T>(v.x * inv);
+            dst[1] = from_float<T>(v.y * inv);
+            dst[2] = from_float<T>(v.z * inv);
+            dst[3] = from_float<T>(v.w * inv);
         } else {
-            s_co[kEven ? 0 : h][d] = v;
-            if (d == 0) {
-                s_cm[h] = m;
-                s_cl[h] = l;
-            }
+            float *p = part + h * kPart;
+            *reinterpret_cast<float4 *>(p + d) = v;
+            if (d == 0) *reinterpret_cast<float2 *>(p + D) = make_float2(s_cm[h], s_cl[h]);
         }
     }
     if (!kEven && a.cluster > 1) {
@@ -721,7 +738,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
                 l += lc * f;
                 v += ld_cluster(&s_co[kEven ? 0 : h][d], c) * f;
             }
-            put(h, d, m, l, v);
+            reinterpret_cast<T *>(a.out)[(long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d] =
+                from_float<T>(l > 0.f || l != l ? v / l : 0.f);
         }
         cluster_sync_all();  // no CTA leaves while its part is read
     }
@@ -729,8 +747,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
     if (nh > 0 && !whole && a.tickets) {
         __shared__ int s_last;
         const int n = units + kSegCost;
-        const long long s0 = (long long)s_prefix[row] * HC + (long long)hc * n;
-        const int c0 = kv8_owner(s0 + kSegCost, runs, total), c1 = kv8_owner(s0 + n - 1, runs, total);
+        const int s0 = s_prefix[row] * HC + hc * n;
+        const int c0 = runs.owner(s0 + kSegCost), c1 = runs.owner(s0 + n - 1);
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -819,11 +837,12 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(T *__restrict__ out, long
     pdl_wait();
     pdl_trigger();
     const int p0 = prefix[row], n = prefix[row + 1] - p0;
-    const long long total = (long long)prefix[rows] * HC;
+    const int total = prefix[rows] * HC;
     if (n == 0) return;
-    const long long runs = kv8_runs(total, ctas), s0 = (long long)p0 * HC + (long long)hc * n;
+    const Kv8Runs cut(total, ctas);
+    const int s0 = p0 * HC + hc * n;
     // the runs with its first and its last step
-    const int c0 = kv8_owner(s0 + kSegCost, runs, total), c1 = kv8_owner(s0 + n - 1, runs, total);
+    const int c0 = cut.owner(s0 + kSegCost), c1 = cut.owner(s0 + n - 1);
     if (c0 == c1) return;  // one run had all of it
     // the first run's part begins with the head group, the others continue it
     const float *base = part + ((long)c0 * 2 * HB + hl % HB) * (D + 4);
@@ -873,7 +892,7 @@ struct Kv8Split {
     int ctas;  // even shares (0: clusters)
     bool wide;  // even shares: more than 16 parts to a head group, which a second launch joins
 };
-Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sms) {
+Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads, int D, int sms) {
     Kv8Split s;
     const int G = heads / kv_heads;
     s.ng = G <= 8 ? 1 : 2;
@@ -888,7 +907,10 @@ Kv8Split kv8_split(int rows, int max_len, int heads, int kv_heads, int D, int sm
     if (want > useful) want = useful;
     s.cluster = want >= 8 ? 8 : (int)want;
     s.wide = pairs * 16 < ctas;
-    s.ctas = rows <= kEvenMaxRows && pairs * units > WK_EVENMIN * ctas ? (int)ctas : 0;
+    // (costs are added up in 32 bits)
+    s.ctas = rows <= kEvenMaxRows && pairs * units > WK_EVENMIN * ctas &&
+                     pairs * (2l * max_pages + kSegCost) < (1l << 30) && ctas <= kTickets
+                 ? (int)ctas : 0;
     return s;
 }
 long long kv8_ws_bytes(const Kv8Split &s, int rows, int D) {
@@ -986,7 +1008,7 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
 long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim) {
     if (rows < 1 || max_len < 1 || kv_heads < 1 || n_heads < 1 || n_heads % kv_heads || head_dim < 1) return 0;
     const int sms = g_rt.num_sms > 0 ? g_rt.num_sms : 148;
-    return kv8_ws_bytes(kv8_split(rows, max_len, n_heads, kv_heads, head_dim, sms), rows, head_dim);
+    return kv8_ws_bytes(kv8_split(rows, max_len, 1, n_heads, kv_heads, head_dim, sms), rows, head_dim);
 }
 
 int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
@@ -1008,7 +1030,7 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     if ((uintptr_t)ws % 16) return fail("wk_kv8_attention: workspace must be 16-byte aligned");
     if (g_rt.device < 0) return fail("wk_kv8_attention: cuda_init() has not been called");
     DeviceGuard guard;
-    Kv8Split sp = kv8_split(rows, max_len, n_heads, kv_heads, head_dim, g_rt.num_sms);
+    Kv8Split sp = kv8_split(rows, max_len, max_pages, n_heads, kv_heads, head_dim, g_rt.num_sms);
     if (!ws || ws_bytes < kv8_ws_bytes(sp, rows, head_dim)) sp.ctas = 0;
     Kv8Attn a;
     a.out = out;
