@@ -249,10 +249,10 @@ __device__ __forceinline__ f32x2 pk_add2(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// the largest of three, NaN if one is
+// the largest of three (of those that are not NaN)
 __device__ __forceinline__ float pk_max3(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ float pk_ex2(float x) {
@@ -666,7 +666,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 }
                 half(0, true, m, sum, pv);
                 const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                if (mb != mb) l = mb;  // a key that this row sees scores NaN: so does the row
                 const bool move = (mb - m) * a.scale_log2 > 8.f || (m == -INFINITY && mb > m);
                 if (__any_sync(0xffffffffu, move)) {
                     const float mn = move ? mb : m;
