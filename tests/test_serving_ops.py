@@ -117,10 +117,12 @@ def _refused(call, words):
     (dict(n=0), "n 0"), (dict(n=8193), "n 8193"), (dict(rows_cap=-1), "bad sizes"), (dict(max_pages=0), "bad sizes"),
     (dict(free_cap=-1), "bad sizes"), (dict(n=8192, max_pages=1 << 20), "2^31"), (dict(starts=None), "null"),
     (dict(row_pos=None), "null"), (dict(n_free=None), "null"), (dict(free_pages=None), "null"),
+    (dict(ctx=2 * FAKE + 2), "misaligned"), (dict(row_slot=FAKE + 4), "misaligned"), (dict(lens=2 * FAKE), "must not be"),
+    (dict(starts=3 * FAKE), "must not be"),
 ])
 def test_plan_refusals(change, words):
     a = dict(starts=FAKE, lens=FAKE, row_seq=FAKE, row_pos=FAKE, row_slot=None, rows_cap=8, table=FAKE, max_pages=4,
-             status=FAKE, ctx=FAKE, add=FAKE, n=2, free_pages=FAKE, n_free=FAKE, free_cap=3)
+             status=FAKE, ctx=2 * FAKE, add=3 * FAKE, n=2, free_pages=FAKE, n_free=FAKE, free_cap=3)
     a.update(change)
     _refused(lambda L: L.wk_batch_plan(*a.values()), words)
 
@@ -129,7 +131,7 @@ def test_plan_refusals(change, words):
     (dict(n=-1), "bad sizes"), (dict(rows=-1), "bad sizes"), (dict(n_pages=0), "bad sizes"),
     (dict(kv_heads=0), "bad sizes"), (dict(hd=96), "head_dim 96"), (dict(dt=wk.F32), "dtype 0"),
     (dict(k=None), "null"), (dict(vscale=None), "null"), (dict(k_rs=127), "stride"), (dict(v_rs=0), "stride"),
-    (dict(kpool=FAKE + 8), "aligned"),
+    (dict(kpool=FAKE + 8), "aligned"), (dict(k=FAKE + 1), "misaligned"), (dict(vscale=FAKE + 2), "misaligned"),
 ])
 def test_store_refusals(change, words):
     a = dict(kpool=FAKE, vpool=FAKE, kscale=FAKE, vscale=FAKE, n_pages=9, k=FAKE, k_rs=128, v=FAKE, v_rs=128,
@@ -143,7 +145,8 @@ def test_store_refusals(change, words):
     (dict(ws_bytes=-1), "bad sizes"), (dict(heads=3), "3 heads over 2"), (dict(heads=0), "heads"),
     (dict(hd=32), "head_dim 32"), (dict(dt=wk.Q8_0), "dtype 8"), (dict(q=None), "null"), (dict(pos=None), "null"),
     (dict(q_rs=255), "stride"), (dict(out_rs=1), "stride"), (dict(vpool=FAKE + 4), "aligned"),
-    (dict(ws=FAKE + 4, ws_bytes=99), "workspace"),
+    (dict(ws=FAKE + 4, ws_bytes=99), "workspace"), (dict(max_pages=1 << 26), "bad sizes"),
+    (dict(q=FAKE + 1), "misaligned"), (dict(pos=FAKE + 2), "misaligned"),
 ])
 def test_decode_refusals(change, words):
     a = dict(out=FAKE, out_rs=256, q=FAKE, q_rs=256, kpool=FAKE, vpool=FAKE, kscale=FAKE, vscale=FAKE, n_pages=4,
@@ -157,7 +160,8 @@ def test_decode_refusals(change, words):
     (dict(n=-1), "bad sizes"), (dict(q_rows=-1), "bad sizes"), (dict(k_rows=-1), "bad sizes"),
     (dict(heads=5), "5 heads over 2"), (dict(kv_heads=0), "heads"), (dict(hd=80), "head_dim 80"),
     (dict(dt=wk.F32), "dtype 0"), (dict(out=None), "null"), (dict(k=None), "null"), (dict(k_starts=None), "null"),
-    (dict(v_rs=127), "stride"), (dict(out_rs=255), "stride"),
+    (dict(v_rs=127), "stride"), (dict(out_rs=255), "stride"), (dict(out=FAKE + 1), "misaligned"),
+    (dict(q_starts=FAKE + 2), "misaligned"),
 ])
 def test_packed_refusals(change, words):
     a = dict(out=FAKE, out_rs=256, q=FAKE, q_rs=256, k=FAKE, k_rs=128, v=FAKE, v_rs=128, q_starts=FAKE, k_starts=FAKE,
@@ -714,6 +718,9 @@ def test_packed_without_keys(dev, shift):
     ([150000], 4, 1, 64, wk.F16),                            # one row: a second launch joins the parts
     ([70000, 0, 70000], 40, 2, 128, wk.BF16),
     ([5] * 2100, 2, 1, 64, wk.F16),                          # more rows than equal runs take
+    ([0, 1800, -1, 900, 33, 0, 1200, 64] * 8, 16, 8, 128, wk.F16),
+    ([2500, 1, 30, 70] * 25, 32, 2, 128, wk.BF16),
+    (list(range(1, 2600, 33)), 8, 8, 64, wk.BF16),
 ])
 def test_decode_shares(dev, lens, heads, kv, hd, dt):
     c = make_decode([n - 1 for n in lens], heads, kv, hd, dt, seed=len(lens) + hd)
@@ -728,12 +735,12 @@ def test_decode_shares(dev, lens, heads, kv, hd, dt):
 def test_decode_workspace_serves_calls_of_other_sizes(dev):
     """One workspace through calls of different shapes, in turn, each as from a fresh one."""
     cases = [make_decode([n - 1 for n in lens], *shape, seed=7) for lens, shape in (
-        (list(range(3, 2400, 57)), (8, 2, 64, wk.F16)), ([150000], (4, 1, 64, wk.F16)),
-        ([4000, 1, 30, 70] * 5, (32, 2, 128, wk.F16)))]
+        ([0, 1800, -1, 900, 33, 0, 1200, 64] * 8, (16, 8, 128, wk.F16)), ([150000], (4, 1, 64, wk.F16)),
+        ([2500, 1, 30, 70] * 25, (32, 2, 128, wk.F16)), (list(range(1, 2600, 33)), (8, 8, 64, wk.F16)))]
     n = max(dev.wk_kv8_attention_ws(len(c["pos"]), int(c["pos"].max()) + 1, c["heads"], c["kv"], c["hd"]) for c in cases)
     ws = up(np.zeros(n, np.uint8))
-    for c in [*cases, *cases[::-1]]:
-        want, tol = ref_decode(c)
+    wants = [ref_decode(c) for c in cases]
+    for c, (want, tol) in [*zip(cases, wants), *zip(cases[::-1], wants[::-1])]:
         rows, w = c["q"].shape
         b = [up(v) for v in (np.zeros((rows, w), np.float16), to_bits(c["q"], c["dt"]), *c["codes"],
                              *(s.astype(np.float32) for s in c["scales"]), c["table"].astype(np.int32),

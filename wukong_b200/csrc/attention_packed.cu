@@ -90,7 +90,9 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 //   O_t += P_t V   (TMEM, fp32)       l_t += row sums of P_t before rounding
 // m is a maximum that is moved, and O_t and l_t scaled, only when it falls more
 // than 2^8 behind the running maximum: p <= 2^8 keeps its relative rounding, and
-// nearly every block skips the pass over O_t.
+// nearly every block skips the pass over O_t.  The first half of a block's
+// exponentials is computed against the old maximum before the block's own is
+// known, and thrown away in the rare case that it moves.
 //   warps 0-3, 4-7   softmax of tile 0, tile 1 (one thread per row), epilogue
 //   warp 8           issues the tcgen05.mma
 //   warp 9           TMA: Q, then K and V blocks through a ring
@@ -106,6 +108,17 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // Where the units are fewer than half the SMs, a cluster of CTAs takes each, with
 // consecutive shares of its key blocks, and joins O, m and l through distributed
 // shared memory.
+//
+// What bounds it: one block of two tiles takes 3200 to 3400 cycles with D = 128, of
+// which the tensor cores run 2048 and the exponentials fill their pipe for 2048;
+// the two overlap except where S, P and the barriers between them change hands
+// (a barrier's answer waits 150 to 350 cycles behind queued exponentials).  8192 x 32
+// heads of 128 over 8: 440 us, 1250 TFLOP/s; behind a long context the tensor pipe is
+// active 62 % of the time.  Measured and not kept: exponentials on the FMA pipe by
+// a polynomial for 1/8 to 1/2 of the keys (no faster), an issuing warp per tile (the
+// tiles fall in phase, 16 % slower), P in TMEM columns of its own for D = 64 (the same
+// time), one tile per CTA and two CTAs per SM (25 % slower at 8192), persistent
+// CTAs over units (24 ragged prompts 5 % faster, one of 8192 3 % slower).
 constexpr int kPkThreads = 384;
 constexpr int kPkRegs = 168;  // registers per thread at launch
 constexpr int kPkKeys = 128;  // keys per block
@@ -429,173 +442,173 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         const int part = max(0, (shift + j0 + 1) / kPkKeys);  // blocks below this are seen whole by every row
         // registers: 256 softmax threads x 216 + 128 x 72 = the launch's 384 x 168
         if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 9) {
-            if (nb > 0 && pk_elect()) {
-                const uint32_t qbytes = (uint32_t)(PT * a.GT) * D * 2;
-                auto load_q = [&](int t) {
-                    for (int b = 0; b < D / 64; ++b)
-                        pk_tma3(smem + L::kQ + t * L::kTile + b * 16384, &maps.q, 64 * b, head0, q0 + j0 + t * PT,
-                                &B->q_full);
-                };
-                mbar_expect_tx(&B->q_full, n0 > 0 && n1 > 0 ? 2 * qbytes : qbytes);
-                if (n0 > 0) load_q(0);
-                auto raw = [&](int i) -> uint64_t * {
-                    return (i & 1) && (i >> 1) >= part ? &B->v_raw[((i >> 1) - part) & 3] : nullptr;
-                };
-                int issued = 0;
-                for (int i = 0; i < 2 * nb; ++i) {
-                    const int s = i % ST;
-                    if (i >= ST && !pk_wait(&B->kv_empty[s], ((i / ST) - 1) & 1, a.err, 50)) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+            if (warp == 9) {
+                if (nb > 0 && pk_elect()) {
+                    const uint32_t qbytes = (uint32_t)(PT * a.GT) * D * 2;
+                    auto load_q = [&](int t) {
+                        for (int b = 0; b < D / 64; ++b)
+                            pk_tma3(smem + L::kQ + t * L::kTile + b * 16384, &maps.q, 64 * b, head0, q0 + j0 + t * PT,
+                                    &B->q_full);
+                    };
+                    mbar_expect_tx(&B->q_full, n0 > 0 && n1 > 0 ? 2 * qbytes : qbytes);
+                    if (n0 > 0) load_q(0);
+                    auto raw = [&](int i) -> uint64_t * {
+                        return (i & 1) && (i >> 1) >= part ? &B->v_raw[((i >> 1) - part) & 3] : nullptr;
+                    };
+                    int issued = 0;
+                    for (int i = 0; i < 2 * nb; ++i) {
+                        const int s = i % ST;
+                        if (i >= ST && !pk_wait(&B->kv_empty[s], ((i / ST) - 1) & 1, a.err, 50)) {
+                            ok = false;
+                            break;
+                        }
+                        uint64_t *bar = &B->kv_full[s];
+                        if (raw(i)) {  // lands on a barrier of its own; the ring's only keeps step
+                            pk_arrive(bar);
+                            bar = raw(i);
+                        }
+                        mbar_expect_tx(bar, L::kTile);
+                        const CUtensorMap *m = (i & 1) ? &maps.v : &maps.k;
+                        for (int b = 0; b < D / 64; ++b)
+                            pk_tma3(smem + L::kRing + (size_t)s * L::kTile + b * 16384, m, 64 * b, kvh,
+                                    k0 + (i >> 1) * kPkKeys, bar);
+                        ++issued;
+                        if (i == 0 && n1 > 0) load_q(1);
+                    }
+                    if (!ok)  // no copy of this CTA may land after it has left
+                        for (int i = max(0, issued - ST); i < issued; ++i) {
+                            if (raw(i))
+                                pk_wait(raw(i), (((i >> 1) - part) >> 2) & 1, a.err, 51);
+                            else
+                                pk_wait(&B->kv_full[i % ST], (i / ST) & 1, a.err, 51);
+                        }
+                }
+            } else if (warp == 8) {
+                if (nb > 0 && pk_elect()) {
+                    constexpr uint32_t fmt = (1u << 4) | (PkType<T>::fmt << 7) | (PkType<T>::fmt << 10) | (8u << 24);
+                    constexpr uint32_t id_qk = fmt | (uint32_t)(kPkKeys >> 3) << 17;
+                    constexpr uint32_t id_pv = fmt | (1u << 16) | (uint32_t)(D >> 3) << 17;  // B (V) MN-major
+                    const uint32_t ring = smem_u32(smem + L::kRing), qs = smem_u32(smem + L::kQ);
+                    // the halves of a descriptor: the upper is constant, the lower the address
+                    const uint32_t q_lo = (uint32_t)pk_desc(qs, 16), ring_lo = (uint32_t)pk_desc(ring, 16);
+                    constexpr uint32_t hi = (uint32_t)(1024 >> 4) | 1u << 14 | 2u << 29;
+                    constexpr uint32_t mn = (uint32_t)(16384 >> 4) << 16;  // V: leading offset of the next 64 dimensions
+                    constexpr uint32_t step = L::kTile >> 4;
+                    auto qk = [&](int t, int stage) {
+                        const uint32_t kb = ring_lo + stage * step, qb = q_lo + t * step;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t o = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                            pk_mma_ss(tmem + t * 128, pk_join(qb + o, hi), pk_join(kb + o, hi), id_qk, kk != 0);
+                        }
+                        pk_commit(&B->s_full[t]);
+                    };
+                    auto pv = [&](int t, int stage, int half, uint32_t acc) {
+                        const uint32_t vb = (ring_lo & 0xffffu) + stage * step + mn + half * (4 * 2048 >> 4);
+                        const uint32_t pb = tmem + t * 128 + 32 * half;
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            pk_mma_ts(tmem + 256 + t * 128, pb + 8 * kk, pk_join(vb + kk * (2048 >> 4), hi), id_pv, acc | kk);
+                    };
+                    // A wait costs 150 to 200 cycles even when its barrier is done (it queues behind
+                    // the softmax warps' exponentials), so the waits for K and V come while the first
+                    // tile's softmax still runs, and the commits that nobody waits for come last.
+                    int stage = 0;
+                    uint32_t phase = 0;
+                    auto next = [&]() {
+                        if (++stage == ST) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    };
+                    ok = pk_wait(&B->q_full, 0, a.err, 53) && pk_wait(&B->kv_full[0], 0, a.err, 52);
+                    if (ok) {
+                        pk_fence_after();
+                        if (n0 > 0) qk(0, 0);
+                        if (n1 > 0) qk(1, 0);
+                        pk_commit(&B->kv_empty[0]);
+                    }
+                    next();
+#pragma unroll 1
+                    for (int j = 0; j < nb && ok; ++j) {
+                        const int vs = stage;
+                        ok = pk_wait(&B->kv_full[vs], phase, a.err, 52);
+                        if (j >= part) ok = ok && pk_wait(&B->v_clean[(j - part) & 3], ((j - part) >> 2) & 1, a.err, 54);
+                        next();
+                        const int ks = stage;
+                        if (j + 1 < nb) ok = ok && pk_wait(&B->kv_full[ks], phase, a.err, 52);
+                        next();
+#pragma unroll 1
+                        for (int t = 0; t < 2; ++t) {
+                            const int nt = t ? n1 : n0;
+                            if (j < nt) {
+                                ok = ok && pk_wait(&B->p_half[t], j & 1, a.err, 55);
+                                if (!ok) break;
+                                pk_fence_after();
+                                pv(t, vs, 0, j);
+                                ok = pk_wait(&B->p_full[t], j & 1, a.err, 60);
+                                if (!ok) break;
+                                pk_fence_after();
+                                pv(t, vs, 1, 1);
+                                if (j + 1 == nt) pk_commit(&B->o_full[t]);
+                            }
+                            if (j + 1 < nt) qk(t, ks);
+                        }
+                        if (ok) {
+                            pk_commit(&B->kv_empty[vs]);
+                            if (j + 1 < nb) pk_commit(&B->kv_empty[ks]);
+                        }
+                    }
+                }
+            } else {
+                // ---- V of the blocks that are seen in part
+                const int ct = tid - 320;  // 0..63
+                for (int j = part; j < nb && ok; ++j) {
+                    const int s = (2 * j + 1) % ST, c = j - part;
+                    if (!pk_wait(&B->v_raw[c & 3], (c >> 2) & 1, a.err, 56)) {
                         ok = false;
                         break;
                     }
-                    uint64_t *bar = &B->kv_full[s];
-                    if (raw(i)) {  // lands on a barrier of its own; the ring's only keeps step
-                        pk_arrive(bar);
-                        bar = raw(i);
-                    }
-                    mbar_expect_tx(bar, L::kTile);
-                    const CUtensorMap *m = (i & 1) ? &maps.v : &maps.k;
-                    for (int b = 0; b < D / 64; ++b)
-                        pk_tma3(smem + L::kRing + (size_t)s * L::kTile + b * 16384, m, 64 * b, kvh,
-                                k0 + (i >> 1) * kPkKeys, bar);
-                    ++issued;
-                    if (i == 0 && n1 > 0) load_q(1);
-                }
-                if (!ok)  // no copy of this CTA may land after it has left
-                    for (int i = max(0, issued - ST); i < issued; ++i) {
-                        if (raw(i))
-                            pk_wait(raw(i), (((i >> 1) - part) >> 2) & 1, a.err, 51);
-                        else
-                            pk_wait(&B->kv_full[i % ST], (i / ST) & 1, a.err, 51);
-                    }
-            }
-        } else if (warp == 8) {
-            if (nb > 0 && pk_elect()) {
-                constexpr uint32_t fmt = (1u << 4) | (PkType<T>::fmt << 7) | (PkType<T>::fmt << 10) | (8u << 24);
-                constexpr uint32_t id_qk = fmt | (uint32_t)(kPkKeys >> 3) << 17;
-                constexpr uint32_t id_pv = fmt | (1u << 16) | (uint32_t)(D >> 3) << 17;  // B (V) MN-major
-                const uint32_t ring = smem_u32(smem + L::kRing), qs = smem_u32(smem + L::kQ);
-                // the halves of a descriptor: the upper is constant, the lower the address
-                const uint32_t q_lo = (uint32_t)pk_desc(qs, 16), ring_lo = (uint32_t)pk_desc(ring, 16);
-                constexpr uint32_t hi = (uint32_t)(1024 >> 4) | 1u << 14 | 2u << 29;
-                constexpr uint32_t mn = (uint32_t)(16384 >> 4) << 16;  // V: leading offset of the next 64 dimensions
-                constexpr uint32_t step = L::kTile >> 4;
-                auto qk = [&](int t, int stage) {
-                    const uint32_t kb = ring_lo + stage * step, qb = q_lo + t * step;
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t o = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-                        pk_mma_ss(tmem + t * 128, pk_join(qb + o, hi), pk_join(kb + o, hi), id_qk, kk != 0);
-                    }
-                    pk_commit(&B->s_full[t]);
-                };
-                auto pv = [&](int t, int stage, int half, uint32_t acc) {
-                    const uint32_t vb = (ring_lo & 0xffffu) + stage * step + mn + half * (4 * 2048 >> 4);
-                    const uint32_t pb = tmem + t * 128 + 32 * half;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        pk_mma_ts(tmem + 256 + t * 128, pb + 8 * kk, pk_join(vb + kk * (2048 >> 4), hi), id_pv, acc | kk);
-                };
-                // A wait costs 150 to 200 cycles even when its barrier is done (it queues behind
-                // the softmax warps' exponentials), so the waits for K and V come while the first
-                // tile's softmax still runs, and the commits that nobody waits for come last.
-                int stage = 0;
-                uint32_t phase = 0;
-                auto next = [&]() {
-                    if (++stage == ST) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                };
-                ok = pk_wait(&B->q_full, 0, a.err, 53) && pk_wait(&B->kv_full[0], 0, a.err, 52);
-                if (ok) {
-                    pk_fence_after();
-                    if (n0 > 0) qk(0, 0);
-                    if (n1 > 0) qk(1, 0);
-                    pk_commit(&B->kv_empty[0]);
-                }
-                next();
+                    uint8_t *vb = smem + L::kRing + (size_t)s * L::kTile;
+                    const int live = min(kPkKeys, kl - j * kPkKeys);
+                    // 16-byte chunks: chunk c of key row r lies at place c ^ (r & 7) of its 128 bytes
+                    constexpr uint32_t e = PkType<T>::exp_one;
+                    uint4 *vq = reinterpret_cast<uint4 *>(vb) + ct;
 #pragma unroll 1
-                for (int j = 0; j < nb && ok; ++j) {
-                    const int vs = stage;
-                    ok = pk_wait(&B->kv_full[vs], phase, a.err, 52);
-                    if (j >= part) ok = ok && pk_wait(&B->v_clean[(j - part) & 3], ((j - part) >> 2) & 1, a.err, 54);
-                    next();
-                    const int ks = stage;
-                    if (j + 1 < nb) ok = ok && pk_wait(&B->kv_full[ks], phase, a.err, 52);
-                    next();
-#pragma unroll 1
-                    for (int t = 0; t < 2; ++t) {
-                        const int nt = t ? n1 : n0;
-                        if (j < nt) {
-                            ok = ok && pk_wait(&B->p_half[t], j & 1, a.err, 55);
-                            if (!ok) break;
-                            pk_fence_after();
-                            pv(t, vs, 0, j);
-                            ok = pk_wait(&B->p_full[t], j & 1, a.err, 60);
-                            if (!ok) break;
-                            pk_fence_after();
-                            pv(t, vs, 1, 1);
-                            if (j + 1 == nt) pk_commit(&B->o_full[t]);
+                    for (int q = 0; q < kPkKeys * D / 8; q += 8 * 64) {
+                        uint4 u[8];
+                        uint32_t hit = 0;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) u[x] = vq[q + 64 * x];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const int r = ((ct + q + 64 * x) >> 3) & 127;
+                            if (r >= live)
+                                vq[q + 64 * x] = make_uint4(0, 0, 0, 0);
+                            else
+                                hit |= ((u[x].x & 0x7fff7fffu) + e) | ((u[x].y & 0x7fff7fffu) + e) |
+                                       ((u[x].z & 0x7fff7fffu) + e) | ((u[x].w & 0x7fff7fffu) + e);
                         }
-                        if (j + 1 < nt) qk(t, ks);
-                    }
-                    if (ok) {
-                        pk_commit(&B->kv_empty[vs]);
-                        if (j + 1 < nb) pk_commit(&B->kv_empty[ks]);
-                    }
-                }
-            }
-        } else {
-            // ---- V of the blocks that are seen in part
-            const int ct = tid - 320;  // 0..63
-            for (int j = part; j < nb && ok; ++j) {
-                const int s = (2 * j + 1) % ST, c = j - part;
-                if (!pk_wait(&B->v_raw[c & 3], (c >> 2) & 1, a.err, 56)) {
-                    ok = false;
-                    break;
-                }
-                uint8_t *vb = smem + L::kRing + (size_t)s * L::kTile;
-                const int live = min(kPkKeys, kl - j * kPkKeys);
-                // 16-byte chunks: chunk c of key row r lies at place c ^ (r & 7) of its 128 bytes
-                constexpr uint32_t e = PkType<T>::exp_one;
-                uint4 *vq = reinterpret_cast<uint4 *>(vb) + ct;
+                        if (hit & 0x80008000u) {  // rare
+                            unsigned short *v = reinterpret_cast<unsigned short *>(vq + q);
 #pragma unroll 1
-                for (int q = 0; q < kPkKeys * D / 8; q += 8 * 64) {
-                    uint4 u[8];
-                    uint32_t hit = 0;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) u[x] = vq[q + 64 * x];
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const int r = ((ct + q + 64 * x) >> 3) & 127;
-                        if (r >= live)
-                            vq[q + 64 * x] = make_uint4(0, 0, 0, 0);
-                        else
-                            hit |= ((u[x].x & 0x7fff7fffu) + e) | ((u[x].y & 0x7fff7fffu) + e) |
-                                   ((u[x].z & 0x7fff7fffu) + e) | ((u[x].w & 0x7fff7fffu) + e);
-                    }
-                    if (hit & 0x80008000u) {  // rare
-                        unsigned short *v = reinterpret_cast<unsigned short *>(vq + q);
-#pragma unroll 1
-                        for (int y = 0; y < 64; ++y) {
-                            const int x = y >> 3, c = ct + q + 64 * x, r = (c >> 3) & 127;
-                            unsigned short *w = v + 64 * 8 * x + (y & 7);
-                            if (r < live && ((*w & 0x7fffu) + (e & 0xffffu)) & 0x8000u) {
-                                *w = 0;
-                                atomicMin(&B->bad_key[(c >> 10) * 64 + ((c & 7) ^ (r & 7)) * 8 + (y & 7)],
-                                          j * kPkKeys + r);
-                                B->bad = 1;
+                            for (int y = 0; y < 64; ++y) {
+                                const int x = y >> 3, c = ct + q + 64 * x, r = (c >> 3) & 127;
+                                unsigned short *w = v + 64 * 8 * x + (y & 7);
+                                if (r < live && ((*w & 0x7fffu) + (e & 0xffffu)) & 0x8000u) {
+                                    *w = 0;
+                                    atomicMin(&B->bad_key[(c >> 10) * 64 + ((c & 7) ^ (r & 7)) * 8 + (y & 7)],
+                                              j * kPkKeys + r);
+                                    B->bad = 1;
+                                }
                             }
                         }
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    pk_arrive(&B->v_clean[c & 3]);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                pk_arrive(&B->v_clean[c & 3]);
             }
-        }
         } else {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
             // ---- softmax: thread = row of tile t
@@ -849,15 +862,15 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     constexpr size_t smem = L::kBars + sizeof(PkBars<D>) + 1024;
     static_assert(smem <= 232448, "shared memory of a CTA");
     auto kern = attn_packed_kernel<T, D>;
-    static bool configured = false;
-    if (!configured) {
+    static int configured = -1;  // the device that the kernel is set up for
+    if (configured != g_rt.device) {
         cudaFuncAttributes fa;
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);
         if (e != cudaSuccess) return e;
         if (fa.numRegs != kPkRegs) return cudaErrorInvalidKernelImage;  // the register split would not add up
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
-        configured = true;
+        configured = g_rt.device;
     }
     PkArgs a;
     a.out = p.out;
@@ -880,7 +893,8 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     const long long units = most < p.q_rows ? most : p.q_rows;
     const long long ctas = units * p.kv_heads * a.chunks;
     // Few units and long sequences: a cluster to each, with two blocks of keys or more per CTA
-    // (1 prompt of 2000 rows behind 14000, 8 heads over 1: 63 units alone SPLIT_FIGURES).
+    // (1 prompt of 2000 rows behind 14000, 8 heads over 1, 63 units: 225 us with a CTA each, 127 to
+    // 155 with two, as the clock allows).
     long long split = g_rt.num_sms / ctas, blocks = p.k_rows / ((long long)kPkKeys * p.n);
     if (split > blocks / 2) split = blocks / 2;
     a.split = split < 2 ? 1 : split > 8 ? 8 : (int)split;
@@ -937,6 +951,9 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
     const long qw = (long)n_heads * head_dim, kw = (long)kv_heads * head_dim;
     if (out_rs < qw || q_rs < qw || k_rs < kw || v_rs < kw)
         return fail("wk_attention_packed: row stride below heads * head_dim");
+    if ((((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 2) ||
+        (((uintptr_t)q_starts | (uintptr_t)k_starts) % 4))
+        return fail("wk_attention_packed: misaligned argument");
     if (g_rt.device < 0) return fail("wk_attention_packed: cuda_init() has not been called");
     DeviceGuard guard;
     PackedArgs a{out, out_rs, q, k, v, q_rs, k_rs, v_rs, q_starts, k_starts, n, q_rows, k_rows, n_heads, kv_heads,

@@ -177,17 +177,23 @@ int wk_batch_plan(int *starts, int *lens, int *row_seq, int *row_pos, long long 
     if (!starts || !lens || !block_table || !status || !ctx || !add || !n_free || (rows_cap && (!row_seq || !row_pos)) ||
         (free_cap && !free_pages))
         return fail("wk_batch_plan: null argument");
+    const uintptr_t low = (uintptr_t)starts | (uintptr_t)lens | (uintptr_t)row_seq | (uintptr_t)row_pos |
+                          (uintptr_t)block_table | (uintptr_t)status | (uintptr_t)ctx | (uintptr_t)add |
+                          (uintptr_t)free_pages | (uintptr_t)n_free;
+    if (low % 4 || (uintptr_t)row_slot % 8) return fail("wk_batch_plan: misaligned argument");
+    if (lens == ctx || lens == add || starts == ctx || starts == add)
+        return fail("wk_batch_plan: starts and lens must not be the arrays of the lengths");
     if (g_rt.device < 0) return fail("wk_batch_plan: cuda_init() has not been called");
     DeviceGuard guard;
     PlanArgs a{starts, lens, row_seq, row_pos, row_slot, rows_cap, block_table, max_pages,
                status, ctx,  add,     n,       free_pages, n_free, free_cap};
     const size_t smem = sizeof(int) * (4 * (size_t)n + 2);
-    static size_t smem_set = 48 * 1024;
-    if (smem > smem_set) {
+    static int configured = -1;  // the device that the kernel is set up for
+    if (smem > 48 * 1024 && configured != g_rt.device) {
         cudaError_t e = cudaFuncSetAttribute(batch_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)(sizeof(int) * (4 * (size_t)kPlanMaxSeqs + 2)));
         if (e != cudaSuccess) return fail("wk_batch_plan: %s", cudaGetErrorString(e));
-        smem_set = sizeof(int) * (4 * (size_t)kPlanMaxSeqs + 2);
+        configured = g_rt.device;
     }
     // one thread per row (or sequence), at most one CTA per SM
     const int work = rows_cap > n ? rows_cap : n;

@@ -210,9 +210,6 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 //             them to arrive joins the parts in their order (a second launch does, where
 //             they are many)
 constexpr int kAtWarps = 4;
-#ifndef WK_EVENMIN
-#define WK_EVENMIN 8
-#endif
 constexpr int kAtKeys = 32;  // keys per warp and step
 
 // CTAs that an SM holds, by their registers.
@@ -245,10 +242,8 @@ struct Kv8Attn {
 // its start and its end (lengths, table, first K and V, queries, the join of the
 // warps) being worth kSegCost steps; one without keys costs nothing.  The sum
 // `total` of the costs is cut into runs, run c being [c total / runs, (c + 1) total / runs).
-#ifndef WK_SEGCOST
-#define WK_SEGCOST 8
-#endif
-constexpr int kSegCost = WK_SEGCOST;
+// (64 rows of 130 to 8191 keys, 8 K/V heads: 69.2 us with 4, 61.4 with 8, 61.6 with 16.)
+constexpr int kSegCost = 8;
 constexpr int kTickets = 4096;  // at most so many CTAs
 struct Kv8Runs {
     int total, runs, q, r;
@@ -892,7 +887,7 @@ struct Kv8Split {
     int ctas;  // even shares (0: clusters)
     bool wide;  // even shares: more than 16 parts to a head group, which a second launch joins
 };
-Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads, int D, int sms) {
+Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads, int D, int sms, bool workspace) {
     Kv8Split s;
     const int G = heads / kv_heads;
     s.ng = G <= 8 ? 1 : 2;
@@ -900,17 +895,25 @@ Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads
     const long pairs = (long)rows * kv_heads * s.chunks;
     const int units = max_len > 0 ? (max_len - 1) / kAtKeys + 1 : 1;
     const long ctas = (long)kv8_per_sm(s.ng, D) * sms;
-    const int useful = (units + kAtWarps - 1) / kAtWarps;          // CTAs with a step for every warp
-    long want = ctas / pairs > 0 ? ctas / pairs : 1;               // fill the machine, in one wave
-    const int tail = (units + 16 * kAtWarps - 1) / (16 * kAtWarps);  // at most 16 steps per warp
-    if (want < tail) want = tail;
-    if (want > useful) want = useful;
-    s.cluster = want >= 8 ? 8 : (int)want;
+    // Clusters: as many CTAs each as fill the machine in one wave and have a step for every
+    // warp.  Equal runs where that leaves a warp more than 12 steps in a row, or rows to wait
+    // for one another in waves (a wave's steps are then many, too).  us, clusters / runs:
+    //   16 rows of 4096, 8 K/V heads (11 steps)   28.9 / 32.0     8 of 2048   13.2 / 17.6
+    //   1 row of 16384, 8 heads (16 steps)        25.5 / 19.8     1 of 32768, 1 head   44.0 / 15.5
+    //   64 rows of 130 to 8191, 8 heads           81.2 / 53.5     64 of 1024  34.2 / 34.2
+    const int useful = (units + kAtWarps - 1) / kAtWarps;
+    const long one_wave = ctas / pairs > 0 ? ctas / pairs : 1;
+    const long most = useful < 8 ? useful : 8;
+    auto clamp = [&](long c) -> int { return (int)(c < most ? c : most); };
+    s.cluster = clamp(one_wave);
+    // a pair's parts are joined by the last run to arrive, up to 16 of them on average
     s.wide = pairs * 16 < ctas;
     // (costs are added up in 32 bits)
-    s.ctas = rows <= kEvenMaxRows && pairs * units > WK_EVENMIN * ctas &&
+    s.ctas = workspace && rows <= kEvenMaxRows && units > 12l * kAtWarps * s.cluster &&
                      pairs * (2l * max_pages + kSegCost) < (1l << 30) && ctas <= kTickets
                  ? (int)ctas : 0;
+    // clusters all the same: at most 16 steps per warp, as far as 8 CTAs go
+    if (!s.ctas && clamp(units / (16 * kAtWarps) + 1) > s.cluster) s.cluster = clamp(units / (16 * kAtWarps) + 1);
     return s;
 }
 long long kv8_ws_bytes(const Kv8Split &s, int rows, int D) {
@@ -988,6 +991,9 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
     if (k_rs < (long)kv_heads * head_dim || v_rs < (long)kv_heads * head_dim)
         return fail("wk_kv8_store: row stride below kv_heads * head_dim");
     if (((uintptr_t)kpool % 16) || ((uintptr_t)vpool % 16)) return fail("wk_kv8_store: pools must be 16-byte aligned");
+    if ((((uintptr_t)k | (uintptr_t)v) % 2) ||
+        (((uintptr_t)kscale | (uintptr_t)vscale | (uintptr_t)starts | (uintptr_t)ctx | (uintptr_t)block_table) % 4))
+        return fail("wk_kv8_store: misaligned argument");
     if (g_rt.device < 0) return fail("wk_kv8_store: cuda_init() has not been called");
     DeviceGuard guard;
     Kv8Store a{{(uint8_t *)kpool, (uint8_t *)vpool}, {kscale, vscale}, n_pages, {k, v}, {k_rs, v_rs}, starts, ctx, n,
@@ -1008,14 +1014,15 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
 long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim) {
     if (rows < 1 || max_len < 1 || kv_heads < 1 || n_heads < 1 || n_heads % kv_heads || head_dim < 1) return 0;
     const int sms = g_rt.num_sms > 0 ? g_rt.num_sms : 148;
-    return kv8_ws_bytes(kv8_split(rows, max_len, 1, n_heads, kv_heads, head_dim, sms), rows, head_dim);
+    return kv8_ws_bytes(kv8_split(rows, max_len, 1, n_heads, kv_heads, head_dim, sms, true), rows, head_dim);
 }
 
 int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
                      const float *kscale, const float *vscale, int n_pages, const int *block_table, int n_seqs,
                      int max_pages, const int *seq, const int *pos, int rows, int max_len, int n_heads, int kv_heads,
                      int head_dim, int dtype, void *ws, long long ws_bytes) {
-    if (rows < 0 || rows > 65535 || n_pages < 1 || n_seqs < 1 || max_pages < 1 || max_len < 0 || ws_bytes < 0)
+    if (rows < 0 || rows > 65535 || n_pages < 1 || n_seqs < 1 || max_pages < 1 || max_pages > 1 << 25 ||
+        max_len < 0 || ws_bytes < 0)
         return fail("wk_kv8_attention: bad sizes");
     if (kv_heads < 1 || n_heads < 1 || n_heads % kv_heads) return fail("wk_kv8_attention: %d heads over %d", n_heads, kv_heads);
     if (head_dim != 64 && head_dim != 128) return fail("wk_kv8_attention: head_dim %d (64 or 128)", head_dim);
@@ -1028,10 +1035,14 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     if (((uintptr_t)kpool % 16) || ((uintptr_t)vpool % 16))
         return fail("wk_kv8_attention: pools must be 16-byte aligned");
     if ((uintptr_t)ws % 16) return fail("wk_kv8_attention: workspace must be 16-byte aligned");
+    if ((((uintptr_t)out | (uintptr_t)q) % 2) ||
+        (((uintptr_t)kscale | (uintptr_t)vscale | (uintptr_t)block_table | (uintptr_t)seq | (uintptr_t)pos) % 4))
+        return fail("wk_kv8_attention: misaligned argument");
     if (g_rt.device < 0) return fail("wk_kv8_attention: cuda_init() has not been called");
     DeviceGuard guard;
-    Kv8Split sp = kv8_split(rows, max_len, max_pages, n_heads, kv_heads, head_dim, g_rt.num_sms);
-    if (!ws || ws_bytes < kv8_ws_bytes(sp, rows, head_dim)) sp.ctas = 0;
+    Kv8Split sp = kv8_split(rows, max_len, max_pages, n_heads, kv_heads, head_dim, g_rt.num_sms, ws != nullptr);
+    if (ws_bytes < kv8_ws_bytes(sp, rows, head_dim))
+        sp = kv8_split(rows, max_len, max_pages, n_heads, kv_heads, head_dim, g_rt.num_sms, false);
     Kv8Attn a;
     a.out = out;
     a.out_rs = out_rs;
