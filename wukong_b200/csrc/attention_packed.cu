@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 constexpr int kPkThreads = 384;
 constexpr int kPkRegs = 168;  // registers per thread at launch
 constexpr int kPkKeys = 128;  // keys per block
+constexpr int kPkGridY = 32768;  // units go over the grid's y, then z
 
 template <int D> struct PkLayout {
     static constexpr int kTile = 128 * D * 2;                 // bytes of a Q tile or a K / V block
@@ -131,12 +132,18 @@ template <int D> struct PkLayout {
     static constexpr size_t kBars = kRing + (size_t)kStages * kTile;
 };
 
+struct PkUnit {
+    int valid;
+    int q0, ql, k0, kl;  // the sequence's first rows and their counts
+    int j0;              // first query of the unit
+};
+
 template <int D> struct PkBars {
     uint64_t q_full, kv_full[PkLayout<D>::kStages], kv_empty[PkLayout<D>::kStages];
     uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
     uint64_t v_raw[4], v_clean[4];  // V blocks that are seen in part: loaded, cleared (the ring holds at most 4)
     uint32_t tmem;
-    int found[6];      // sequence, unit within it, its first query and key rows and their counts
+    PkUnit unit;
     int units[kPkThreads / 32];
     int bad;           // a non-finite V in a masked block
     __align__(16) int bad_key[D];  // first key that holds one, per dimension
@@ -301,7 +308,8 @@ struct PkArgs {
     void *out;
     long out_rs;
     const int *q_starts, *k_starts;
-    int n, q_rows, k_rows, G, GT, chunks, kv_heads;  // heads per K/V head, heads per tile, tiles of heads per K/V head
+    int n, q_rows, k_rows, G, GT, chunks;  // heads per K/V head, heads per tile, tiles of heads per K/V head
+    int PT;                                // positions per tile
     float scale_log2;
     int vec;  // out is 16-byte aligned and strided
     int split;  // CTAs of a cluster, which share a unit's keys
@@ -340,96 +348,131 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     PkBars<D> *B = reinterpret_cast<PkBars<D> *>(smem + L::kBars);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in the whole warp
-    if (tid == 0) {
-        mbar_init(&B->q_full, 1);
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(&B->kv_full[i], 1);
-            mbar_init(&B->kv_empty[i], 1);
+    if (warp == 9) {  // the loading warp, which waits for nobody before its first loads
+        if (lane == 0) {
+            mbar_init(&B->q_full, 1);
+            for (int i = 0; i < ST; ++i) {
+                mbar_init(&B->kv_full[i], 1);
+                mbar_init(&B->kv_empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&B->s_full[i], 1);
+                mbar_init(&B->p_half[i], 128);
+                mbar_init(&B->p_full[i], 128);
+                mbar_init(&B->o_full[i], 1);
+            }
+            for (int i = 0; i < 4; ++i) {
+                mbar_init(&B->v_raw[i], 1);
+                mbar_init(&B->v_clean[i], 64);
+            }
+            mbar_fence_init();
+        } else if (lane < 4) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 1 ? &maps.q : lane == 2 ? &maps.k : &maps.v) : "memory");
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&B->s_full[i], 1);
-            mbar_init(&B->p_half[i], 128);
-            mbar_init(&B->p_full[i], 128);
-            mbar_init(&B->o_full[i], 1);
-        }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&B->v_raw[i], 1);
-            mbar_init(&B->v_clean[i], 64);
-        }
-        mbar_fence_init();
-        B->found[0] = -1;
-        B->bad = 0;
-    }
-    for (int i = tid; i < D; i += kPkThreads) B->bad_key[i] = 0x7fffffff;
-    if (warp == 8) {
+        __syncwarp();
+    } else if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B->tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == 9 && lane < 3)
-        asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v) : "memory");
+    if (tid == 0) {
+        B->unit.valid = 0;
+        B->bad = 0;
+    }
+    if (tid < D) B->bad_key[tid] = 0x7fffffff;
     pk_fence_before();
     pdl_wait();
     pdl_trigger();
     // ---- this CTA's unit: the idx-th from the end, so that the longest rows of a long prompt start first
-    const int rank = blockIdx.x % a.split, bid = blockIdx.x / a.split;
-    const int hb = bid % (a.kv_heads * a.chunks), idx = bid / (a.kv_heads * a.chunks);
-    const int kvh = hb / a.chunks, chunk = hb % a.chunks;
-    const int PT = 128 / a.GT;
-    int before = 0;
-    for (int i0 = 0; i0 < a.n; i0 += kPkThreads) {
-        const int i = a.n - 1 - (i0 + tid);
-        int u = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-        if (i >= 0) {
-            q0 = a.q_starts[i];
-            q1 = a.q_starts[i + 1];
-            k0 = a.k_starts[i];
-            k1 = a.k_starts[i + 1];
-            q0 = min(max(q0, 0), a.q_rows);
-            q1 = min(max(q1, q0), a.q_rows);
-            k0 = min(max(k0, 0), a.k_rows);
-            k1 = min(max(k1, k0), a.k_rows);
-            u = (q1 - q0 + 2 * PT - 1) / (2 * PT);
+    const int idx = blockIdx.z * kPkGridY + blockIdx.y;
+    const int rank = a.split == 1 ? 0 : blockIdx.x % a.split, hb = a.split == 1 ? blockIdx.x : blockIdx.x / a.split;
+    const int kvh = a.chunks == 1 ? hb : hb / a.chunks, chunk = a.chunks == 1 ? 0 : hb % a.chunks;
+    const int PT = a.PT;
+    PkUnit unit = {0, 0, 0, 0, 0, 0};
+    // sequence i, counted from the end, and its units
+    auto look = [&](int i, int &units) -> PkUnit {
+        PkUnit s = {0, 0, 0, 0, 0, 0};
+        units = 0;
+        if (i < a.n) {
+            i = a.n - 1 - i;
+            const int q0 = a.q_starts[i], q1 = a.q_starts[i + 1], k0 = a.k_starts[i], k1 = a.k_starts[i + 1];
+            s.q0 = min(max(q0, 0), a.q_rows);
+            s.ql = min(max(q1, s.q0), a.q_rows) - s.q0;
+            s.k0 = min(max(k0, 0), a.k_rows);
+            s.kl = min(max(k1, s.k0), a.k_rows) - s.k0;
+            units = (s.ql + 2 * PT - 1) / (2 * PT);
         }
-        int in = u;
+        return s;
+    };
+    if (a.n <= 32) {
+        // the loading warp for itself, warp 0 for the others
+        if (warp == 9 || warp == 0) {
+            int units;
+            const PkUnit s = look(lane, units);
+            int in = units;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, in, o);
-            if (lane >= o) in += v;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, in, o);
+                if (lane >= o) in += v;
+            }
+            const uint32_t who = __ballot_sync(0xffffffffu, idx >= in - units && idx < in);
+            if (who) {
+                const int from = __ffs(who) - 1;
+                unit.valid = 1;
+                unit.q0 = __shfl_sync(0xffffffffu, s.q0, from);
+                unit.ql = __shfl_sync(0xffffffffu, s.ql, from);
+                unit.k0 = __shfl_sync(0xffffffffu, s.k0, from);
+                unit.kl = __shfl_sync(0xffffffffu, s.kl, from);
+                unit.j0 = (__shfl_sync(0xffffffffu, in, from) - 1 - idx) * 2 * PT;
+                if (warp == 0 && lane == 0) B->unit = unit;
+            }
+        }
+        if (warp == 9)
+            asm volatile("bar.arrive 2, %0;" ::"n"(kPkThreads) : "memory");
+        else
+            asm volatile("bar.sync 2, %0;" ::"n"(kPkThreads) : "memory");
+    } else {
+        int before = 0;
+        for (int i0 = 0; i0 < a.n; i0 += kPkThreads) {
+            int units;
+            PkUnit s = look(i0 + tid, units);
+            int in = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, in, o);
+                if (lane >= o) in += v;
+            }
+            __syncthreads();
+            if (lane == 31) B->units[warp] = in;
+            __syncthreads();
+            int first = before + in - units;
+#pragma unroll
+            for (int w = 0; w < kPkThreads / 32; ++w) {
+                if (w < warp) first += B->units[w];
+                before += B->units[w];
+            }
+            if (idx >= first && idx < first + units) {
+                s.valid = 1;
+                s.j0 = (units - 1 - (idx - first)) * 2 * PT;
+                B->unit = s;
+            }
+            if (idx < before) break;
         }
         __syncthreads();
-        if (lane == 31) B->units[warp] = in;
-        __syncthreads();
-        int first = before + in - u;
-#pragma unroll
-        for (int w = 0; w < kPkThreads / 32; ++w) {
-            if (w < warp) first += B->units[w];
-            before += B->units[w];
-        }
-        if (idx >= first && idx < first + u) {
-            B->found[0] = i;
-            B->found[1] = u - 1 - (idx - first);
-            B->found[2] = q0;
-            B->found[3] = q1 - q0;
-            B->found[4] = k0;
-            B->found[5] = k1 - k0;
-        }
-        if (idx < before) break;
     }
-    __syncthreads();
+    if (warp != 9 || a.n > 32) unit = B->unit;
     pk_fence_after();
     const uint32_t tmem = B->tmem;
-    const int seq = B->found[0];
     bool ok = true;
-    if (seq >= 0) {
-        const int q0 = B->found[2], ql = B->found[3];
-        const int j0 = B->found[1] * 2 * PT;      // first query of the unit
+    if (unit.valid) {
+        const int q0 = unit.q0, ql = unit.ql;
+        const int j0 = unit.j0;  // first query of the unit
         const int head0 = kvh * a.G + chunk * a.GT;
         // The unit's last query sees `all` blocks of keys; this CTA's share of them starts at
         // block `skip`, and from here on keys count from there.
-        const int all = max(0, (B->found[5] - ql + min(j0 + 2 * PT, ql) - 1 + kPkKeys) / kPkKeys);
-        const int share = (all + a.split - 1) / a.split, skip = rank * share;
-        const int k0 = B->found[4] + skip * kPkKeys, kl = B->found[5] - skip * kPkKeys;
+        const int all = max(0, (unit.kl - ql + min(j0 + 2 * PT, ql) - 1 + kPkKeys) / kPkKeys);
+        const int share = a.split == 1 ? all : (all + a.split - 1) / a.split, skip = rank * share;
+        const int k0 = unit.k0 + skip * kPkKeys, kl = unit.kl - skip * kPkKeys;
         const int shift = kl - ql;  // query j sees keys 0 .. shift + j
         // blocks of keys that each tile sees (0: none), and the first that some row of the unit sees in part
         auto blocks = [&](int t) -> int {
@@ -741,9 +784,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             // Where row x of tile s goes (null: nowhere).  (The unit is read again from shared
             // memory, which keeps the loop over the blocks free of what only the end needs.)
             auto row_out = [&](int s, int x) -> T * {
-                const int j = B->found[1] * 2 * PT + s * PT + x / a.GT, h = chunk * a.GT + x % a.GT;
-                if (x >= PT * a.GT || j >= B->found[3] || h >= a.G || !ok) return nullptr;
-                return reinterpret_cast<T *>(a.out) + (long)(B->found[2] + j) * a.out_rs + (long)(kvh * a.G + h) * D;
+                const PkUnit &un = B->unit;
+                const int j = un.j0 + s * PT + x / a.GT, h = chunk * a.GT + x % a.GT;
+                if (x >= PT * a.GT || j >= un.ql || h >= a.G || !ok) return nullptr;
+                return reinterpret_cast<T *>(a.out) + (long)(un.q0 + j) * a.out_rs + (long)(kvh * a.G + h) * D;
             };
             if (a.split == 1) {
                 // The warp's rows through the part of the Q tile that they came from (all products
@@ -883,7 +927,7 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     a.G = p.heads / p.kv_heads;
     a.GT = GT;
     a.chunks = (a.G + GT - 1) / GT;
-    a.kv_heads = p.kv_heads;
+    a.PT = 128 / GT;
     a.scale_log2 = p.scale * 1.4426950408889634f;
     a.vec = ((uintptr_t)p.out % 16) == 0 && p.out_rs % 8 == 0;
     a.err = g_rt.d_error;
@@ -898,9 +942,10 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     long long split = g_rt.num_sms / ctas, blocks = p.k_rows / ((long long)kPkKeys * p.n);
     if (split > blocks / 2) split = blocks / 2;
     a.split = split < 2 ? 1 : split > 8 ? 8 : (int)split;
-    if (ctas * a.split > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    const long long z = (units + kPkGridY - 1) / kPkGridY;
+    if ((long long)p.kv_heads * a.chunks * a.split > 0x7fffffffll || z > 65535) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ctas * a.split));
+    cfg.gridDim = dim3(p.kv_heads * a.chunks * a.split, (unsigned)(units < kPkGridY ? units : kPkGridY), (unsigned)z);
     cfg.blockDim = dim3(kPkThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
