@@ -161,7 +161,7 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
 /* wk_attention_decode over that cache: row r is a token of sequence seq[r] at
  * position pos[r] and sees the keys 0 .. pos[r]; a row whose seq is outside
  * [0, n_seqs), or whose pos is negative, gets zeros.  Several rows may share a
- * sequence.  n_heads a multiple of kv_heads; head_dim 64 or 128; dtype of q and
+ * sequence; at most 65535 rows.  n_heads a multiple of kv_heads; head_dim 64 or 128; dtype of q and
  * out F16 or BF16; strides in elements.  max_len (the longest pos + 1) only
  * chooses how the work is split.  ws [ws_bytes] is the caller's workspace (16-byte
  * aligned): zeroed by the caller before its first use, left fit for the next

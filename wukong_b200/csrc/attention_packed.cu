@@ -1023,7 +1023,7 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
         e = head_dim == 64 ? launch_rows<__half, 64>(a, s) : launch_rows<__half, 128>(a, s);
     else
         e = head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(a, s) : launch_rows<__nv_bfloat16, 128>(a, s);
-    if (e != cudaSuccess) return fail("wk_attention_packed: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return fail_cuda("wk_attention_packed", e);
     return 0;
 }
 

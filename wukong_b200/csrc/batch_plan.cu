@@ -192,7 +192,7 @@ int wk_batch_plan(int *starts, int *lens, int *row_seq, int *row_pos, long long 
     if (smem > 48 * 1024 && configured != g_rt.device) {
         cudaError_t e = cudaFuncSetAttribute(batch_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)(sizeof(int) * (4 * (size_t)kPlanMaxSeqs + 2)));
-        if (e != cudaSuccess) return fail("wk_batch_plan: %s", cudaGetErrorString(e));
+        if (e != cudaSuccess) return fail_cuda("wk_batch_plan", e);
         configured = g_rt.device;
     }
     // one thread per row (or sequence), at most one CTA per SM
@@ -210,7 +210,7 @@ int wk_batch_plan(int *starts, int *lens, int *row_seq, int *row_pos, long long 
     cfg.attrs = attr;
     cfg.numAttrs = g_rt.pdl ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, batch_plan_kernel, a);
-    if (e != cudaSuccess) return fail("wk_batch_plan: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return fail_cuda("wk_batch_plan", e);
     return 0;
 }
 

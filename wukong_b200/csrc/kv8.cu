@@ -1007,7 +1007,7 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
         e = head_dim == 64 ? launch_store<__half, 64>(a, units, s) : launch_store<__half, 128>(a, units, s);
     else
         e = head_dim == 64 ? launch_store<__nv_bfloat16, 64>(a, units, s) : launch_store<__nv_bfloat16, 128>(a, units, s);
-    if (e != cudaSuccess) return fail("wk_kv8_store: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return fail_cuda("wk_kv8_store", e);
     return 0;
 }
 
@@ -1077,7 +1077,7 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     else
         e = head_dim == 64 ? launch_attn<__nv_bfloat16, 64>(a, sp.ng, s)
                            : launch_attn<__nv_bfloat16, 128>(a, sp.ng, s);
-    if (e != cudaSuccess) return fail("wk_kv8_attention: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return fail_cuda("wk_kv8_attention", e);
     return 0;
 }
 

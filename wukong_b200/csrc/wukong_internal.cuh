@@ -308,6 +308,11 @@ template <typename T> int allreduce_resid(T *x, float *p, long n, cudaStream_t s
 // ---------------------------------------------------------------- engine.cu
 // Records the message returned by wk_last_error() and returns -1.
 int fail(const char *fmt, ...);
+// The same for a refused launch; the error does not wait for the next call's check.
+inline int fail_cuda(const char *who, cudaError_t e) {
+    cudaGetLastError();
+    return fail("%s: %s", who, cudaGetErrorString(e));
+}
 
 // Makes the library's device current for one entry point and puts the caller's back.
 struct DeviceGuard {
