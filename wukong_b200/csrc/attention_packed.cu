@@ -88,6 +88,8 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // K/V tile loaded once serves all of them.  Per block of 128 keys and tile t:
 //   S_t = Q_t K^T  (TMEM, fp32)       P_t = exp2(c (S_t - m))  (16 bits, over S_t in TMEM)
 //   O_t += P_t V   (TMEM, fp32)       l_t += row sums of P_t before rounding
+// P is rounded to V's type, which is what the tensor cores multiply V with: at most
+// half a step of that type relative to each p, and l_t does not inherit it.
 // m is a maximum that is moved, and O_t and l_t scaled, only when it falls more
 // than 2^8 behind the running maximum: p <= 2^8 keeps its relative rounding, and
 // nearly every block skips the pass over O_t.  The first half of a block's

@@ -70,7 +70,12 @@ template <typename T> __device__ __forceinline__ uint32_t to_e4m3x2(uint32_t w, 
 // One CTA per (page that the call writes, K/V head): threads 0..127 take K,
 // 128..255 V.  The page's new rows stay in registers, as the 16-bit values that
 // they are, between the maximum and the rounding, so each is read once; their
-// loads are under way while the block table is read.
+// loads are under way while the block table is read.  Bytes bound long prompts: 9
+// of 301 to 2303 tokens, 8 heads of 128, take 13.9 us, 73 % of the copy rate; what is
+// left is the chain lengths -> table -> old scale -> rows of each CTA, which six CTAs
+// per SM (their register limit) hide in part.  Latency bounds a step of 48 tokens: 7.7 us,
+// 3.3 us in a graph.  VEC: rows whose base and stride are multiples of 16 bytes are
+// read 16 bytes at a time, others element by element (any alignment of the type).
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
     constexpr int kChunks = D / 8;               // 8-element chunks per row
