@@ -715,8 +715,8 @@ def test_packed_without_keys(dev, shift):
     (list(range(3, 2400, 57)), 8, 2, 64, wk.F16),            # equal runs, parts joined by the last to arrive
     ([0, 1800, -1, 900, 33, 0, 1200, 64] * 4, 32, 8, 128, wk.BF16),
     ([4000, 1, 30, 70] * 5, 32, 2, 128, wk.F16),             # 16 heads per K/V head; long rows among short ones
-    ([150000], 4, 1, 64, wk.F16),                            # one row: a second launch joins the parts
-    ([70000, 0, 70000], 40, 2, 128, wk.BF16),
+    ([150000], 4, 1, 64, wk.F16),                            # one row: several clusters to a head group
+    ([70000, 0, 70000], 40, 2, 128, wk.BF16),                # a second launch joins the parts
     ([5] * 2100, 2, 1, 64, wk.F16),                          # more rows than equal runs take
     ([0, 1800, -1, 900, 33, 0, 1200, 64] * 8, 16, 8, 128, wk.F16),
     ([2500, 1, 30, 70] * 25, 32, 2, 128, wk.BF16),
@@ -729,6 +729,28 @@ def test_decode_shares(dev, lens, heads, kv, hd, dt):
     close(got, want, tol)
     assert np.array_equal(got, run_decode(dev, c, max(lens), ws=True))
     close(run_decode(dev, c, max(lens), ws=False), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,heads,kv,hd,dt", [
+    (16383, 32, 8, 128, wk.BF16),
+    (40001, 7, 1, 128, wk.F16),   # 7 heads: the last CTA of a cluster joins fewer outputs
+    (9000, 40, 4, 128, wk.F16),   # 10 heads per K/V head, in one CTA
+    (19000, 40, 4, 128, wk.BF16),
+    (20000, 24, 1, 64, wk.BF16),  # 24 of them, in two
+    (33000, 3, 3, 64, wk.F16),
+])
+def test_decode_one_long_row(dev, n, heads, kv, hd, dt):
+    """Several clusters to a head group; the row as long as announced, much shorter, a padding row."""
+    c = make_decode([n - 1], heads, kv, hd, dt, seed=n)
+    need = dev.wk_kv8_attention_ws(1, n, heads, kv, hd)
+    for pos in (n - 1, 1000, 0, -1):
+        d = dict(c, pos=np.array([pos]))
+        want, tol = ref_decode(d)
+        got = run_decode(dev, d, n, ws=True)
+        close(got, want, tol)
+        assert np.array_equal(got, run_decode(dev, d, n, ws=True))
+        close(run_decode(dev, d, n, short_ws=max(need - 1, 0)), want, tol)
 
 
 @pytest.mark.gpu

@@ -206,9 +206,10 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 // the tensor cores.  e4m3 converts to fp16 exactly; bf16 queries are brought to
 // fp16 by a power of two per head (their largest value to [2^14, 2^15)).
 // A warp takes 32 keys at a time and keeps the next 32 keys' K and V in flight.
-// The context is shared out in one of two ways:
+// The context is shared out in one of these ways:
 //   clusters  a cluster of CTAs takes one (row, K/V head) and joins its parts
-//             (m, l, O) through distributed shared memory: one launch
+//             (m, l, O) through distributed shared memory: one launch.  One long row has
+//             several; the last of them to arrive joins what they left in the workspace
 //   even      the steps of all rows and K/V heads, one after the other, are cut into as
 //             many equal runs as CTAs fit on the GPU; a run that ends inside a
 //             (row, K/V head) leaves its part in the caller's workspace, and the last of
@@ -236,11 +237,13 @@ struct Kv8Attn {
     int vec;       // q rows are 8-byte aligned
     int rows;
     int cluster;   // CTAs that share a (row, K/V head)
+    int groups;    // clusters that share it, their parts meeting in the workspace
     int ctas;      // even shares: CTAs of the launch
-    int *tickets;  // even shares: [kTickets] arrivals of a head group's parts, at the run with its first step; zero
-                   // between calls.  Null: a second launch joins the parts.
+    int *tickets;  // [kTickets] arrivals of a head group's parts, at the run with its first step (groups: at the
+                   // head group); zero between calls.  Null: a second launch joins the parts.
     int *prefix;   // even shares: [rows + 1] cost of the rows before each, per head group (written by CTA 0)
     float *part;   // even shares: [ctas][2][8 NG][D + 4]: O, m, l of a run's part of a head group
+                   // groups: [head groups][groups][8 NG][D + 4]
 };
 
 // Even shares: a (row, head group) of n steps costs n + kSegCost, the latencies of
@@ -316,7 +319,7 @@ template <> struct Kv8Q<__nv_bfloat16> {
     static constexpr bool rescale = true;
 };
 
-// grid: clusters (cluster * chunks * kv_heads, rows); even shares (ctas)
+// grid: clusters (cluster * chunks * kv_heads, rows, groups); even shares (ctas)
 template <typename T, int D, int NG, bool kEven>
 __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_kernel(const Kv8Attn a) {
     constexpr int HB = 8 * NG;       // heads per CTA
@@ -411,9 +414,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
         u1 = cut - kSegCost;
         step = kAtWarps;
     } else {
-        u0 = rank * kAtWarps + warp;
+        u0 = (blockIdx.z * a.cluster + rank) * kAtWarps + warp;
         u1 = units;
-        step = a.cluster * kAtWarps;
+        step = a.groups * a.cluster * kAtWarps;
     }
 
     uint4 kr[4][KC];   // K: rows g, g + 8, g + 16, g + 24 of the step's keys
@@ -727,6 +730,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
         cluster_sync_all();
         const int share = (nh * D + a.cluster - 1) / a.cluster;
         const int x1 = min(nh * D, (rank + 1) * share);
+        T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_rs + (long)(kvh * a.G + h0) * D;
+        float *group0 = a.part + (long)hc * a.groups * HB * kPart;
         for (int x = rank * share + tid; x < x1; x += kAtWarps * 32) {
             const int h = x / D, d = x % D;
             float m = -INFINITY;
@@ -738,8 +743,50 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
                 l += lc * f;
                 v += ld_cluster(&s_co[kEven ? 0 : h][d], c) * f;
             }
-            reinterpret_cast<T *>(a.out)[(long)row * a.out_rs + (long)(kvh * a.G + h0 + h) * D + d] =
-                from_float<T>(l > 0.f || l != l ? v / l : 0.f);
+            if (a.groups > 1) {
+                float *p = group0 + ((long)blockIdx.z * HB + h) * kPart;
+                p[d] = v;
+                if (d == 0) *reinterpret_cast<float2 *>(p + D) = make_float2(m, l);
+            } else {
+                out[h * D + d] = from_float<T>(l > 0.f || l != l ? v / l : 0.f);
+            }
+        }
+        if (a.groups > 1) {
+            // the last cluster to arrive joins the parts, in their order
+            __threadfence();
+            cluster_sync_all();
+            __shared__ float s_last;
+            if (rank == 0 && tid == 0) {
+                const bool last = atomicAdd(&a.tickets[hc], 1) == a.groups - 1;
+                if (last) a.tickets[hc] = 0;
+                s_last = last ? 1.f : 0.f;
+            }
+            cluster_sync_all();
+            if (ld_cluster(&s_last, 0) != 0.f) {
+                __threadfence();
+                float2(*s_ml)[HB] = reinterpret_cast<float2(*)[HB]>(&s_o[0][0][0]);  // [groups][head]
+                for (int x = tid; x < a.groups * HB; x += kAtWarps * 32) {
+                    const int c = x / HB, h = x % HB;
+                    if (h < nh)
+                        s_ml[c][h] = __ldcg(reinterpret_cast<const float2 *>(group0 + ((long)c * HB + h) * kPart + D));
+                }
+                __syncthreads();
+                for (int x = rank * share + tid; x < x1; x += kAtWarps * 32) {
+                    const int h = x / D, d = x % D;
+                    const float *p = group0 + h * kPart + d;
+                    float m = -INFINITY, l = 0.f, v = 0.f;
+                    for (int c = 0; c < a.groups; ++c) m = fmaxf(m, s_ml[c][h].x);
+#pragma unroll 16
+                    for (int c = 0; c < a.groups; ++c) {
+                        const float o = __ldcg(p + c * (HB * kPart));
+                        const float2 ml = s_ml[c][h];
+                        const float f = ml.x == -INFINITY ? (ml.y != ml.y ? 1.f : 0.f) : ex2(ml.x - m);
+                        l += ml.y * f;
+                        v += o * f;
+                    }
+                    out[h * D + d] = from_float<T>(l > 0.f || l != l ? v / l : 0.f);
+                }
+            }
         }
         cluster_sync_all();  // no CTA leaves while its part is read
     }
@@ -887,10 +934,12 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(T *__restrict__ out, long
 
 // How a call's context is shared out.
 constexpr int kEvenMaxRows = 2048;  // their prefix sums lie in shared memory
+constexpr int kMaxGroups = 64;      // their maxima and sums lie in shared memory
 struct Kv8Split {
     int ng, chunks, cluster;
-    int ctas;  // even shares (0: clusters)
-    bool wide;  // even shares: more than 16 parts to a head group, which a second launch joins
+    int groups;  // clusters to a head group
+    int ctas;    // even shares (0: clusters)
+    bool wide;   // even shares: more than 16 parts to a head group, which a second launch joins
 };
 Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads, int D, int sms, bool workspace) {
     Kv8Split s;
@@ -904,7 +953,6 @@ Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads
     // warp.  Equal runs where that leaves a warp more than 12 steps in a row, or rows to wait
     // for one another in waves (a wave's steps are then many, too).  us, clusters / runs:
     //   16 rows of 4096, 8 K/V heads (11 steps)   28.9 / 32.0     8 of 2048   13.2 / 17.6
-    //   1 row of 16384, 8 heads (16 steps)        25.5 / 19.8     1 of 32768, 1 head   44.0 / 15.5
     //   64 rows of 130 to 8191, 8 heads           81.2 / 53.5     64 of 1024  34.2 / 34.2
     const int useful = (units + kAtWarps - 1) / kAtWarps;
     const long one_wave = ctas / pairs > 0 ? ctas / pairs : 1;
@@ -917,13 +965,33 @@ Kv8Split kv8_split(int rows, int max_len, int max_pages, int heads, int kv_heads
     s.ctas = workspace && rows <= kEvenMaxRows && units > 12l * kAtWarps * s.cluster &&
                      pairs * (2l * max_pages + kSegCost) < (1l << 30) && ctas <= kTickets
                  ? (int)ctas : 0;
+    // One row that leaves a cluster's warps more than 4 steps (8 of head_dim 64: with 6, 9.8 us in one
+    // cluster, 10.4 in several): several clusters of 8 to a head
+    // group, until a warp has 1 step (head_dim 64) or 2 (128: 8192 keys, 32 / 8 heads take
+    // 14.5 us with 2, 15.2 with 1; 16384 keys, 16 / 4 heads of 64 12.6 and 10.5), or no more fit
+    // at once (7 of 8 CTAs, for a cluster takes its SMs from one part of the GPU).
+    // us, one cluster or equal runs / several clusters:
+    //   8192 keys, 8 / 1 heads of 128   13.9 / 11.3     32768   15.4 / 12.5    131071   21.2 / 19.0
+    //   8192 keys, 32 / 8 heads of 128  15.8 / 14.5     16384   20.0 / 17.5     65536   34.2 / 32.9
+    s.groups = 1;
+    const long fit = ctas * 7 / 64 / pairs;
+    if (workspace && rows == 1 && fit > 1 && units > (D == 64 ? 8 : 4) * kAtWarps * s.cluster) {
+        const int each = 8 * kAtWarps * (D == 64 ? 1 : 2), want = (units + each - 1) / each;
+        s.cluster = 8;
+        s.groups = (int)(fit < kMaxGroups ? fit : kMaxGroups);
+        if (want < s.groups) s.groups = want;
+        s.ctas = 0;
+        s.wide = false;
+        return s;
+    }
     // clusters all the same: at most 16 steps per warp, as far as 8 CTAs go
     if (!s.ctas && clamp(units / (16 * kAtWarps) + 1) > s.cluster) s.cluster = clamp(units / (16 * kAtWarps) + 1);
     return s;
 }
-long long kv8_ws_bytes(const Kv8Split &s, int rows, int D) {
+long long kv8_ws_bytes(const Kv8Split &s, int rows, int head_groups, int D) {
     const long long prefix = (4ll * (rows + 1) + 15) / 16 * 16;
-    return s.ctas ? 4ll * kTickets + prefix + 4ll * s.ctas * 2 * 8 * s.ng * (D + 4) : 0;
+    const long long parts = s.ctas ? 2ll * s.ctas : s.groups > 1 ? (long long)s.groups * head_groups : 0;
+    return parts ? 4ll * kTickets + prefix + 4ll * parts * 8 * s.ng * (D + 4) : 0;
 }
 
 template <typename T, int D> cudaError_t launch_store(const Kv8Store &a, int units, cudaStream_t s) {
@@ -955,7 +1023,7 @@ template <typename T, int D, int NG> cudaError_t launch_attn_ng(const Kv8Attn &a
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     if (a.ctas == 0) {
-        cfg.gridDim = dim3(a.cluster * a.chunks * a.kv_heads, a.rows);
+        cfg.gridDim = dim3(a.cluster * a.chunks * a.kv_heads, a.rows, a.groups);
         cfg.numAttrs = 2;
         return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, D, NG, false>, a);
     }
@@ -1019,7 +1087,8 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
 long long wk_kv8_attention_ws(int rows, int max_len, int n_heads, int kv_heads, int head_dim) {
     if (rows < 1 || max_len < 1 || kv_heads < 1 || n_heads < 1 || n_heads % kv_heads || head_dim < 1) return 0;
     const int sms = g_rt.num_sms > 0 ? g_rt.num_sms : 148;
-    return kv8_ws_bytes(kv8_split(rows, max_len, 1, n_heads, kv_heads, head_dim, sms, true), rows, head_dim);
+    const Kv8Split sp = kv8_split(rows, max_len, 1, n_heads, kv_heads, head_dim, sms, true);
+    return kv8_ws_bytes(sp, rows, kv_heads * sp.chunks, head_dim);
 }
 
 int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const void *kpool, const void *vpool,
@@ -1046,7 +1115,7 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     if (g_rt.device < 0) return fail("wk_kv8_attention: cuda_init() has not been called");
     DeviceGuard guard;
     Kv8Split sp = kv8_split(rows, max_len, max_pages, n_heads, kv_heads, head_dim, g_rt.num_sms, ws != nullptr);
-    if (ws_bytes < kv8_ws_bytes(sp, rows, head_dim))
+    if (ws_bytes < kv8_ws_bytes(sp, rows, kv_heads * sp.chunks, head_dim))
         sp = kv8_split(rows, max_len, max_pages, n_heads, kv_heads, head_dim, g_rt.num_sms, false);
     Kv8Attn a;
     a.out = out;
@@ -1070,6 +1139,7 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
     a.vec = ((uintptr_t)q % 8) == 0 && q_rs % 4 == 0;
     a.cluster = sp.cluster;
+    a.groups = sp.groups;
     a.rows = rows;
     a.ctas = sp.ctas;
     a.tickets = sp.wide ? nullptr : (int *)ws;
