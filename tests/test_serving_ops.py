@@ -360,6 +360,26 @@ def test_store_is_exact(dev, ctx, add, kv, hd, dt, extra, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,some", [(256, 256), (257, 200), (1000, 900), (70000, 150)])
+@pytest.mark.parametrize("late", [0, 90])
+def test_store_finds_each_sequence(dev, n, some, late):
+    """Many sequences, some without rows, of one token or of several pages; rows of nobody before the first."""
+    rng = np.random.default_rng(n + late)
+    add, ctx = np.zeros(n + 1, int), np.zeros(n + 1, int)
+    on = 1 + np.sort(rng.permutation(n)[:some])
+    add[on] = rng.choice([1, 1, 1, 2, 64, 65, 66, 130], some)
+    ctx[on] = rng.integers(0, 70, some)
+    add[0] = late
+    c = make_store(ctx, add, 1, 64, wk.F16, 0, 0, seed=n)
+    c = dict(c, starts=c["starts"][1:], ctx=c["ctx"][1:], table=c["table"][1:])
+    got = run_store(dev, c)
+    for i in range(2):
+        codes, scales = ref_store(c["old"][i], c["olds"][i], c["x"][i], c["starts"], c["ctx"], c["table"], c["n_pages"])
+        assert np.array_equal(got[2 + i].astype(np.float64), scales)
+        assert same_codes(got[i], codes).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [wk.F16, wk.BF16])
 def test_store_extremes(dev, dt):
     """Zeros, infinities, NaN, the type's largest and smallest values; a page without an id; a table that ends."""

@@ -81,51 +81,42 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
     constexpr int kChunks = D / 8;               // 8-element chunks per row
     constexpr int kRows = 128 / kChunks;         // rows per pass of 128 threads
     constexpr int kPasses = kKv8Page / kRows;
-    __shared__ int s_units[8];
     __shared__ int s_found[5];  // sequence, page index, first row, tokens, first offset
     __shared__ uint32_t s_max[8];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int unit = blockIdx.x, head = blockIdx.y;
     if (tid == 0) s_found[0] = -1;
+    __syncthreads();
     pdl_wait();
     pdl_trigger();
-    // the sequence and page of this CTA: a scan over the pages that each sequence's new tokens touch
-    int before = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 256) {
-        const int i = i0 + tid;
-        int r0 = 0, add = 0, ctx = 0, u = 0;
-        if (i < a.n) {
-            r0 = min(max(a.starts[i], 0), a.rows);
-            add = min(max(a.starts[i + 1], r0), a.rows) - r0;
-            ctx = max(a.ctx[i], 0);
-            if (add > 0) u = (ctx % kKv8Page + add + kKv8Page - 1) / kKv8Page;
-        }
-        int in = u;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, in, o);
-            if (lane >= o) in += v;
-        }
-        __syncthreads();
-        if (lane == 31) s_units[wid] = in;
-        __syncthreads();
-        int first = before + in - u;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            if (w < wid) first += s_units[w];
-            before += s_units[w];
-        }
-        if (unit >= first && unit < first + u) {
-            const int k = unit - first;                           // its k-th touched page
-            const int lo = k ? k * kKv8Page - ctx % kKv8Page : 0;  // tokens before this page
-            const int off = k ? 0 : ctx % kKv8Page;
+    // The sequence and page of this CTA.  `add` tokens touch at most add pages, and at most
+    // add / 64 + 2; so sequence i has room from base(i) = min(starts, starts / 64 + 2 i) to
+    // base(i + 1), and it is found by comparisons alone (a scan over the pages that each touches
+    // took 20.6 us instead of 17.8 for 512 sequences of one token, 8 heads of 128; 1092
+    // instead of 267 for 8192).
+    auto start = [&](int i) -> int { return min(max(a.starts[i], 0), a.rows); };
+    auto base = [&](int r, int i) -> int { return (int)min((long)r, r / kKv8Page + 2l * i); };
+    int lo = 0, len = a.n;
+    while (len > 256) {
+        const int st = (len + 255) / 256, i = lo + tid * st;
+        const int c = __syncthreads_count(tid * st < len && base(start(i), i) <= unit);
+        if (c == 0) return;
+        lo += (c - 1) * st;
+        len = min(st, len - (c - 1) * st);
+    }
+    if (tid < len) {
+        const int i = lo + tid, r0 = start(i), r1 = start(i + 1), ctx = max(a.ctx[i], 0);
+        const int add = r1 - r0, k = unit - base(r0, i);  // its k-th touched page
+        const int open = ctx % kKv8Page;
+        if (k >= 0 && unit < base(r1, i + 1) && k < (open + add + kKv8Page - 1) / kKv8Page && add > 0) {
+            const int before = k ? k * kKv8Page - open : 0;  // tokens before this page
+            const int off = k ? 0 : open;
             s_found[0] = i;
             s_found[1] = ctx / kKv8Page + k;
-            s_found[2] = r0 + lo;
-            s_found[3] = min(kKv8Page - off, add - lo);
+            s_found[2] = r0 + before;
+            s_found[3] = min(kKv8Page - off, add - before);
             s_found[4] = off;
         }
-        if (unit < before) break;
     }
     __syncthreads();
     if (s_found[0] < 0 || s_found[1] >= a.max_pages) return;
@@ -1071,7 +1062,7 @@ int wk_kv8_store(void *kpool, void *vpool, float *kscale, float *vscale, int n_p
     DeviceGuard guard;
     Kv8Store a{{(uint8_t *)kpool, (uint8_t *)vpool}, {kscale, vscale}, n_pages, {k, v}, {k_rs, v_rs}, starts, ctx, n,
                rows, block_table, max_pages, kv_heads};
-    // pages touched: at most one per row, and at most ceil((63 + add) / 64) per sequence
+    // base(n) of the kernel, with all rows
     const long long most = (long long)rows / kKv8Page + 2ll * n;
     const int units = (int)(most < rows ? most : rows);
     cudaStream_t s = stream();
