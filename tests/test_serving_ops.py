@@ -654,6 +654,82 @@ def test_packed_attention(dev, ql, kl, heads, kv, hd, dt, extra, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ql,kl,heads,kv,hd,dt,extra,shift", PACKED)
+def test_packed_attention_beside_a_long_sequence(dev, ql, kl, heads, kv, hd, dt, extra, shift):
+    """The same with a token behind a long context, whose length decides how all of them are computed."""
+    c = make_packed([*ql, 1], [*kl, 250 * (len(kl) + 1)], heads, kv, hd, dt, seed=sum(ql) + heads)
+    want, tol = ref_packed(c)
+    close(run_packed(dev, c, extra, shift), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ql,kl,heads,kv,hd,dt,extra", [
+    ([1] * 9, [1, 2, 3, 4, 60, 64, 65, 100, 130], 4, 1, 128, wk.BF16, 8),
+    ([64, 63, 65, 31, 1, 40], [64, 63, 65, 31, 1, 90], 6, 6, 64, wk.F16, 0),       # one head per K/V head
+    ([33, 100, 7], [33, 100, 7], 15, 3, 64, wk.BF16, 0),                             # 5: units begin inside a position
+    ([20, 50], [100, 5], 64, 1, 128, wk.F16, 64),
+    ([4, 9, 2], [40, 9, 120], 65, 1, 64, wk.F16, 0),
+    ([100], [120], 7, 1, 128, wk.BF16, 0),
+    ([3, 0, 0, 120, 5] * 30, [10, 0, 7, 120, 2] * 30, 4, 2, 64, wk.F16, 0),          # more of them than a CTA has threads
+    ([1, 700, 2] + [1] * 27, [1, 700, 2] + [1] * 27, 4, 2, 128, wk.F16, 0),          # one among them is long
+])
+def test_packed_short_sequences(dev, ql, kl, heads, kv, hd, dt, extra):
+    c = make_packed(ql, kl, heads, kv, hd, dt, seed=len(ql) + hd)
+    want, tol = ref_packed(c)
+    got = run_packed(dev, c, extra)
+    close(got, want, tol)
+    assert np.array_equal(got, run_packed(dev, c, extra))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [wk.F16, wk.BF16])
+def test_packed_short_steep_scores(dev, dt):
+    c = make_packed([70, 20], [110, 20], 4, 2, 128, dt, seed=2, spread=12.0)
+    ramp = np.linspace(0.01, 3.0, 130)[:, None]
+    c["k"] = rounded(np.abs(c["k"]) * ramp, dt)
+    c["q"] = rounded(np.abs(c["q"]), dt)
+    want, tol = ref_packed(c)
+    close(run_packed(dev, c), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_packed_short_later_keys_do_not_touch_earlier_queries(dev, bad, hd):
+    c = make_packed([100, 20], [100, 30], 6, 2, hd, wk.F16, seed=7)
+    want, tol = ref_packed(c)
+    for name in "kv":
+        d = dict(c, **{name: c[name].copy()})
+        d[name][37, 3] = bad  # sequence 0, K/V head 0, dimension 3
+        got = run_packed(dev, d)
+        same = np.ones(want.shape, bool)
+        same[37:100, :3 * hd] = False
+        if name == "v":
+            seen = np.zeros(want.shape, bool)
+            seen[37:100, [3, hd + 3, 2 * hd + 3]] = True
+            assert not np.isfinite(got[seen]).any() and (np.isnan(got[seen]) == np.isnan(bad)).all()
+            same = ~seen
+        assert (np.abs(got - want) <= tol)[same].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift,extra", [(1, 0), (0, 3)])
+def test_packed_short_with_an_output_of_any_alignment(dev, shift, extra):
+    c = make_packed([40, 9], [40, 25], 4, 2, 64, wk.BF16, seed=3)
+    want, tol = ref_packed(c)
+    w = c["q"].shape[1]
+    b = [up(to_bits(c[x], wk.BF16)) for x in "qkv"] + [up(c[x].astype(np.int32)) for x in ("qs", "ks")]
+    out = up(np.full(49 * (w + extra) + shift, 0x3555, np.uint16))
+    wk.check(dev.wk_attention_packed(out + 2 * shift, w + extra, b[0], w, b[1], 128, b[2], 128, b[3], b[4], 2, 49, 65, 4, 2,
+                                     64, wk.BF16))
+    raw = down(out, 49 * (w + extra) + shift, np.uint16)
+    free(*b, out)
+    body = raw[shift:].reshape(49, w + extra)
+    assert (raw[:shift] == 0x3555).all() and (body[:, w:] == 0x3555).all()
+    close(from_bits(np.ascontiguousarray(body[:, :w]).view(RAW[wk.BF16]), wk.BF16), want, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [wk.F16, wk.BF16])
 def test_packed_steep_scores(dev, dt):
     """Scores that differ by hundreds, with the largest at the last keys, so that the running maximum keeps growing."""

@@ -6,6 +6,8 @@
 //   o = sum_k softmax_k(q . k / sqrt(d)) v
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "wukong_ext.h"
 #include "wukong_internal.cuh"
@@ -22,6 +24,7 @@ struct PackedArgs {
     const int *q_starts, *k_starts;
     int n, q_rows, k_rows, heads, kv_heads;
     float scale;
+    bool out4;  // out's rows are 4-byte aligned
 };
 
 // One CTA per (query row, head), 128 threads: a thread scores one key of each
@@ -80,6 +83,286 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
     }
     if (tid < D)
         reinterpret_cast<T *>(a.out)[row * a.out_rs + h * D + tid] = from_float<T>(l > 0.f || l != l ? o / l : 0.f);
+}
+
+// ------------------------------------------------------------------ short sequences
+// A CTA takes 64 rows of one sequence and K/V head, a row being a position and one
+// of the G heads of the group (heads inner, so no row is empty but at a sequence's end);
+// a warp takes 16 of them, with S, P and O in mma.sync fragments:
+//   S = Q K^T     P = exp2(c (S - m) + 8)     O += P V     l += row sums of P before rounding
+// Blocks of 64 keys come through two stages of cp.async.  The contraction of Q K^T runs
+// over dims in the order in which 16-byte pieces of a row fall to the four lanes
+// of a row group, so Q goes from global memory straight into its fragments and a K
+// fragment is one 16-byte read.  P in [0, 2^8] keeps the type's full precision down to
+// 2^-22 of the row's largest p in fp16.
+// Latency bounds it: unit -> Q, K, V -> S -> softmax -> O.  Small CTAs, several to an SM, and
+// no tensor memory, barriers or maps to set up are what it has over the tcgen05 kernel: 100
+// sequences of 40 tokens, 16 / 4 heads of 64, take 10.5 us instead of 22.0.  A further block
+// of 64 keys costs 1.6 us with D = 128, so long sequences are not for it (where they begin
+// to cost more stands at the launch).
+// A row whose result is not finite is computed again over the keys that it sees alone,
+// for a masked key has p = 0, and 0 * NaN is NaN.
+__device__ __forceinline__ float pk_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int D> struct ShLayout {
+    static constexpr int kKeys = 64;
+    static constexpr int kPitchK = 2 * D + 64, kPitchV = 2 * D + 16;  // bytes; reads free of bank conflicts
+    static constexpr int kK = kKeys * kPitchK, kStage = kK + kKeys * kPitchV;
+    static constexpr int kSmem = 2 * kStage;
+};
+
+template <typename T> __device__ __forceinline__ uint32_t sh_pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t sh_pack<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t sh_pack<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void sh_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    if (std::is_same<T, __half>::value)
+        mma_f16(c, a0, a1, a2, a3, b0, b1);
+    else
+        mma_bf16(c, a0, a1, a2, a3, b0, b1);
+}
+__device__ __forceinline__ void sh_cp16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kernel(PackedArgs a) {
+    using L = ShLayout<D>;
+    constexpr int NC = D / 32;  // 16-byte pieces of a row per lane
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ int s_unit[6];  // found, q0, ql, k0, kl, first row
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int kvh = blockIdx.x, G = a.heads / a.kv_heads;
+    const int unit = gridDim.y - 1 - blockIdx.y;  // a long prompt's last rows, which see most, start first
+    if (tid == 0) s_unit[0] = 0;
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    // Sequence i has room for its units from base(i) = min(q_starts, G q_starts / 64 + i) to
+    // base(i + 1) (G <= 64), so it is found by comparisons alone.
+    auto start = [&](int i) -> int { return min(max(a.q_starts[i], 0), a.q_rows); };
+    auto base = [&](int r, int i) -> int { return (int)min((long)r, (long)r * G / 64 + i); };
+    int lo = 0, n = a.n;
+    while (n > 128) {
+        const int st = (n + 127) / 128, i = lo + tid * st;
+        const int c = __syncthreads_count(tid * st < n && base(start(i), i) <= unit);
+        if (c == 0) return;
+        lo += (c - 1) * st;
+        n = min(st, n - (c - 1) * st);
+    }
+    if (tid < n) {
+        const int i = lo + tid, r0 = start(i), r1 = max(start(i + 1), r0), k0 = a.k_starts[i], k1 = a.k_starts[i + 1];
+        const int k = unit - base(r0, i);
+        if (k >= 0 && unit < base(r1, i + 1) && (long)k * 64 < (long)(r1 - r0) * G) {
+            s_unit[0] = 1;
+            s_unit[1] = r0;
+            s_unit[2] = r1 - r0;
+            s_unit[3] = min(max(k0, 0), a.k_rows);
+            s_unit[4] = min(max(k1, s_unit[3]), a.k_rows) - s_unit[3];
+            s_unit[5] = k * 64;
+        }
+    }
+    __syncthreads();
+    if (!s_unit[0]) return;
+    const int q0 = s_unit[1], ql = s_unit[2], k0 = s_unit[3], kl = s_unit[4], x0 = s_unit[5];
+    const int rows = (int)min((long)ql * G - x0, 64l);  // of this unit
+    const int p0 = x0 / G, h0 = x0 - p0 * G;            // position and head of its first row
+    auto seen = [&](int r) -> int { return max(0, min(kl, kl - ql + p0 + (h0 + r) / G + 1)); };  // keys of row r
+    const int blocks = (seen(rows - 1) + L::kKeys - 1) / L::kKeys;
+
+    const uint32_t smem = smem_u32(sm);
+    const T *kp = reinterpret_cast<const T *>(a.k) + (long)k0 * a.k_rs + kvh * D;
+    const T *vp = reinterpret_cast<const T *>(a.v) + (long)k0 * a.v_rs + kvh * D;
+    auto load = [&](int b) {
+        constexpr int per = D / 8;  // 16-byte pieces of a row
+        const uint32_t st = smem + (b & 1) * L::kStage;
+#pragma unroll
+        for (int x = 0; x < L::kKeys * per / 128; ++x) {
+            const int j = (tid + x * 128) / per, c = (tid + x * 128) % per, key = b * L::kKeys + j;
+            const int row = min(key, kl - 1), bytes = key < kl ? 16 : 0;  // rows behind the sequence: zeros
+            sh_cp16(st + j * L::kPitchK + c * 16, kp + row * a.k_rs + c * 8, bytes);
+            sh_cp16(st + L::kK + j * L::kPitchV + c * 16, vp + row * a.v_rs + c * 8, bytes);
+        }
+    };
+    if (blocks > 0) load(0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (blocks > 1) load(1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+
+    // this thread's rows: r, r + 8
+    const int r = warp * 16 + g;
+    uint4 q[2][NC];
+    int len[2];
+    long at[2];  // of the row, in heads of the unit's K/V head
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int x = r + 8 * i, p = (h0 + x) / G, h = h0 + x - p * G;
+        len[i] = x < rows ? seen(x) : 0;
+        const T *src = reinterpret_cast<const T *>(a.q) + (long)(q0 + p0 + p) * a.q_rs + (long)(kvh * G + h) * D + t * 8;
+        at[i] = (long)(q0 + p0 + p) * a.out_rs + (long)(kvh * G + h) * D;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            q[i][c] = x < rows ? *reinterpret_cast<const uint4 *>(src + c * 32) : make_uint4(0, 0, 0, 0);
+    }
+    const int wrows = min(rows - warp * 16, 16);  // of this warp
+    const int wlast = wrows > 0 ? seen(warp * 16 + wrows - 1) : 0, wfirst = wrows > 0 ? seen(warp * 16) : 0;
+    const float c2 = a.scale * 1.4426950408889634f;
+    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+
+    for (int b = 0; b < blocks; ++b) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();
+        const int left = wlast - b * L::kKeys;  // keys from here on that a row of the warp sees
+        if (left > 0) {
+            const uint8_t *ks = sm + (b & 1) * L::kStage;
+            const uint32_t vs = smem + (b & 1) * L::kStage + L::kK;
+            float s[8][4];
+#pragma unroll
+            for (int hb = 0; hb < 8; hb += 4) {  // 32 keys: four sums under way at a time
+#pragma unroll
+                for (int nt = hb; nt < hb + 4; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+                if (hb * 8 < left) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        uint4 k[4];
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt)
+                            k[nt] = *reinterpret_cast<const uint4 *>(ks + ((hb + nt) * 8 + g) * L::kPitchK + (t + 4 * c) * 16);
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt)
+                            sh_mma<T>(s[hb + nt], q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y, k[nt].x, k[nt].y);
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt)
+                            sh_mma<T>(s[hb + nt], q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w, k[nt].z, k[nt].w);
+                    }
+                }
+            }
+            if (b * L::kKeys + L::kKeys > wfirst) {
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (b * L::kKeys + nt * 8 + 2 * t + (e & 1) >= len[e >> 1]) s[nt][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float mx = m[i];
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * i], s[nt][2 * i + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float f = mx == m[i] ? 1.f : pk_ex2((m[i] - mx) * c2);
+                const float ref = mx == -INFINITY ? 0.f : mx * c2 - 8.f;
+                m[i] = mx;
+                l[i] *= f;
+#pragma unroll
+                for (int nt = 0; nt < D / 8; ++nt) o[nt][2 * i] *= f, o[nt][2 * i + 1] *= f;
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt) {
+                    s[nt][2 * i] = pk_ex2(s[nt][2 * i] * c2 - ref);
+                    s[nt][2 * i + 1] = pk_ex2(s[nt][2 * i + 1] * c2 - ref);
+                    l[i] += s[nt][2 * i] + s[nt][2 * i + 1];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j * 16 < left) {
+                    const uint32_t a0 = sh_pack<T>(s[2 * j][0], s[2 * j][1]), a1 = sh_pack<T>(s[2 * j][2], s[2 * j][3]);
+                    const uint32_t a2 = sh_pack<T>(s[2 * j + 1][0], s[2 * j + 1][1]),
+                                   a3 = sh_pack<T>(s[2 * j + 1][2], s[2 * j + 1][3]);
+                    const uint32_t vr = vs + (j * 16 + (lane & 15)) * L::kPitchV + (lane >> 4) * 16;
+#pragma unroll
+                    for (int n4 = 0; n4 < D / 16; n4 += 4) {
+                        uint32_t w[4][4];
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt) ldsm_x4_t(vr + (n4 + nt) * 32, w[nt][0], w[nt][1], w[nt][2], w[nt][3]);
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt) {
+                            sh_mma<T>(o[2 * (n4 + nt)], a0, a1, a2, a3, w[nt][0], w[nt][1]);
+                            sh_mma<T>(o[2 * (n4 + nt) + 1], a0, a1, a2, a3, w[nt][2], w[nt][3]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (b + 2 < blocks) load(b + 2);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    uint32_t bad = 0;  // the warp's rows whose result is not finite
+    T *out = reinterpret_cast<T *>(a.out);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
+        bool fine = true;
+#pragma unroll
+        for (int nt = 0; nt < D / 8; ++nt) {
+            o[nt][2 * i] *= inv;
+            o[nt][2 * i + 1] *= inv;
+            fine = fine && fabsf(o[nt][2 * i]) < INFINITY && fabsf(o[nt][2 * i + 1]) < INFINITY;
+        }
+        const uint32_t no = __ballot_sync(0xffffffffu, !fine);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (no >> (4 * x) & 15u) bad |= 1u << (x + 8 * i);
+        if (r + 8 * i < rows && !(bad >> (g + 8 * i) & 1u)) {
+            T *dst = out + at[i] + 2 * t;
+#pragma unroll
+            for (int nt = 0; nt < D / 8; ++nt) {
+                if (a.out4) {
+                    *reinterpret_cast<uint32_t *>(dst + nt * 8) = sh_pack<T>(o[nt][2 * i], o[nt][2 * i + 1]);
+                } else {
+                    dst[nt * 8] = from_float<T>(o[nt][2 * i]);
+                    dst[nt * 8 + 1] = from_float<T>(o[nt][2 * i + 1]);
+                }
+            }
+        }
+    }
+    for (; bad; bad &= bad - 1) {
+        const int x = warp * 16 + __ffs(bad) - 1;
+        if (x >= rows) break;
+        const int p = (h0 + x) / G, h = h0 + x - p * G, len = seen(x);
+        const long head = (long)(kvh * G + h) * D;
+        const T *qr = reinterpret_cast<const T *>(a.q) + (long)(q0 + p0 + p) * a.q_rs + head;
+        float mr = -INFINITY, lr = 0.f, v[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) v[c] = 0.f;
+        for (int j = 0; j < len; ++j) {
+            float dot = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dot += to_float(qr[lane + 32 * c]) * to_float(kp[j * a.k_rs + lane + 32 * c]);
+            dot = warp_sum(dot) * c2;
+            const float mn = fmaxf(mr, dot), f = mr == mn ? 1.f : pk_ex2(mr - mn);
+            const float w = dot == -INFINITY ? 0.f : pk_ex2(dot - mn);
+            mr = mn;
+            lr = lr * f + w;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) v[c] = v[c] * f + w * to_float(vp[j * a.v_rs + lane + 32 * c]);
+        }
+        T *dst = out + (long)(q0 + p0 + p) * a.out_rs + head;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            dst[lane + 32 * c] = from_float<T>(lr > 0.f || lr != lr ? v[c] / lr : 0.f);
+    }
 }
 
 // ------------------------------------------------------------------ tcgen05 kernel
@@ -276,11 +559,6 @@ __device__ __forceinline__ float pk_max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-__device__ __forceinline__ float pk_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // shared-memory descriptors, 128-byte swizzle: K-major rows of 128 bytes (8-row
 // groups 1024 bytes apart), and MN-major (the contraction runs over the rows;
@@ -963,6 +1241,28 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 
+template <typename T, int D> cudaError_t launch_short(const PackedArgs &a, int units, cudaStream_t s) {
+    auto kern = attn_packed_short_kernel<T, D>;
+    static int configured = -1;
+    if (configured != g_rt.device) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ShLayout<D>::kSmem);
+        if (e != cudaSuccess) return e;
+        configured = g_rt.device;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.kv_heads, units);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = ShLayout<D>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_rt.pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
 template <typename T, int D> cudaError_t launch_rows(const PackedArgs &a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.q_rows, a.heads);
@@ -1004,13 +1304,36 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
     if (g_rt.device < 0) return fail("wk_attention_packed: cuda_init() has not been called");
     DeviceGuard guard;
     PackedArgs a{out, out_rs, q, k, v, q_rs, k_rs, v_rs, q_starts, k_starts, n, q_rows, k_rows, n_heads, kv_heads,
-                 1.0f / sqrtf((float)head_dim)};
+                 1.0f / sqrtf((float)head_dim), (uintptr_t)out % 4 == 0 && out_rs % 2 == 0};
     cudaStream_t s = stream();
     cudaError_t e;
     // TMA wants 16-byte aligned bases and strides; what is not goes row by row
     const uintptr_t low = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v;
     if (low % 16 == 0 && (q_rs | k_rs | v_rs) % 8 == 0 && k_rows > 0) {
         const int G = n_heads / kv_heads, GT = G < 128 ? G : 128;
+        // Short sequences: by their mean length, which is all that is known here, with room for
+        // one that is much longer than the others where there are several.  us, this kernel / tcgen05,
+        // 32 / 8 heads of 128:
+        //   1 of 97           8.0 /  9.3     24 of 16        7.0 / 15.4    24 of 1 to 300 (mean 62)  24.3 / 24.5
+        //   1 of 200         10.1 / 10.4     24 of 73 to 97 23.6 / 26.6    24 of 1 to 500 (97)       42.1 / 32.8
+        //   100 of 16        14.4 / 44.6     400 of 40       129 / 218     6 of 1 to 300 (80)        16.2 / 12.6
+        // 16 / 4 heads of 64:
+        //   1 of 256          7.3 /  9.0     24 of 97        7.9 / 13.3    24 of 1 to 300 (62)       11.5 / 12.9
+        //   100 of 40        10.5 / 22.0     24 of 200      16.9 / 20.7    24 of 1 to 500 (97)       17.5 / 16.7
+        const long long shorter = (head_dim == 64 ? 112 : 64) * (n <= 2 ? 2 : 1);
+        // base(n) of that kernel, with all rows
+        long long units = (long long)q_rows * G / 64 + n;
+        if (units > q_rows) units = q_rows;
+        if (G <= 64 && units <= 65535 && kv_heads <= 65535 && k_rows <= shorter * n) {
+            if (dtype == kF16)
+                e = head_dim == 64 ? launch_short<__half, 64>(a, (int)units, s)
+                                   : launch_short<__half, 128>(a, (int)units, s);
+            else
+                e = head_dim == 64 ? launch_short<__nv_bfloat16, 64>(a, (int)units, s)
+                                   : launch_short<__nv_bfloat16, 128>(a, (int)units, s);
+            if (e != cudaSuccess) return fail_cuda("wk_attention_packed", e);
+            return 0;
+        }
         PkMaps maps;
         if (!pk_map(&maps.q, q, dtype, head_dim, n_heads, q_rows, q_rs, GT, 128 / GT) ||
             !pk_map(&maps.k, k, dtype, head_dim, kv_heads, k_rows, k_rs, 1, kPkKeys) ||
