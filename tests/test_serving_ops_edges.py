@@ -1,0 +1,73 @@
+"""Edges of the serving operators: an attention sink far ahead of the keys that carry the output.
+
+Tolerances.  As in the other file, with what it leaves out: a softmax weight is
+multiplied with V in 16 bits, and in fp16 it is exact to half of 2^-24 at the
+least.  The kernels keep weights of one key that leads its row near 2^11 or
+above, so that this is at most 2^-36 of such a key's weight, and the weights sum
+to at least that of one: 2^-36 sum |v| of the keys that a row sees.  An output in
+fp16 is exact to 2^-25 at the least.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import wukong_b200 as wk
+from tests import test_serving_ops as ops
+from tests.test_serving_ops import CODES, PAGE, UNIT, e4m3_codes, rounded, run_decode
+
+
+def attend(q, k, v, dt):
+    """softmax(q k^T / sqrt(d)) v for one query, and how far off a kernel may be."""
+    d, n = q.shape[-1], len(k)
+    s = k @ q / math.sqrt(d)
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    o, A = p @ v, p @ np.abs(v)
+    S = (np.abs(k) @ np.abs(q)).max() / math.sqrt(d)
+    u = UNIT[dt]
+    tol = u * np.abs(o) + A * (u + 2 * (d * 2.0 ** -24 * S + 2.0 ** -20) + n * 2.0 ** -24) * (1 + u)
+    return o, tol + 2.0 ** -36 * np.abs(v).sum(0) + (2.0 ** -25 if dt == wk.F16 else 0.0)
+
+
+def near(got, want, tol):
+    assert np.isfinite(got).all()
+    print(f"largest error / tolerance {float((np.abs(got - want) / np.maximum(tol, 1e-300)).max()):.3f}")
+    assert (np.abs(got - want) <= tol).all()
+
+
+def sinks(rng, n, hd, gap, every):
+    """Keys with scores near 0, every so many of them one whose score is `gap` for a query of gap / sqrt(hd)
+    throughout and whose V is zero."""
+    k, v = 0.3 * rng.standard_normal((n, hd)), 1000.0 * (1 + 0.3 * rng.standard_normal((n, hd)))
+    k[::every], v[::every] = 1.0, 0.0
+    return k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [12.0, 15.0, 18.0])
+@pytest.mark.parametrize("lens,heads,kv,hd,dt,ws", [
+    ([777], 16, 4, 64, wk.F16, True),
+    ([300, 5, 1, 450, 333] * 6, 16, 8, 128, wk.BF16, False),
+    ([40, 2000, 130, 700] * 8, 32, 2, 128, wk.F16, True),   # 16 heads per K/V head, equal runs
+    ([9000], 8, 1, 128, wk.BF16, True),                     # several clusters to a head group
+])
+def test_decode_keeps_the_weights_behind_a_sink(dev, lens, heads, kv, hd, dt, ws, gap):
+    rng = np.random.default_rng(int(gap) + heads)
+    c = ops.make_decode([n - 1 for n in lens], heads, kv, hd, dt, seed=int(gap))
+    c["scales"] = [np.full_like(c["scales"][0], 2.0 ** -5), np.full_like(c["scales"][1], 2.0 ** 4)]
+    c["q"] = rounded(np.full(c["q"].shape, gap / math.sqrt(hd)), dt)
+    want, tol = np.zeros((len(lens), heads, hd)), np.zeros((len(lens), heads, hd))
+    for r, n in enumerate(lens):
+        pages = c["table"][r, : -(-n // PAGE)]
+        for a in range(kv):
+            kv_values = []
+            for x, values in enumerate(sinks(rng, n, hd, gap, 32)):
+                codes = e4m3_codes(values / c["scales"][x][0, 0])
+                for j, page in enumerate(pages):
+                    part = codes[j * PAGE:(j + 1) * PAGE]
+                    c["codes"][x][page, a, : len(part)] = part
+                kv_values.append(CODES[codes] * c["scales"][x][0, 0])
+            for h in range(a * heads // kv, (a + 1) * heads // kv):
+                want[r, h], tol[r, h] = attend(c["q"][r].reshape(heads, hd)[h], *kv_values, dt)
+    near(run_decode(dev, c, max(lens), ws), want.reshape(len(lens), -1), tol.reshape(len(lens), -1))

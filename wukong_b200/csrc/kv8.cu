@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 // ------------------------------------------------------------------ attention
 // Per row and K/V head, G query heads share the keys, 8 NG of them per CTA:
 //   S^T[keys x heads] = K Q^T    m16n8k16, keys in M, 8 heads in N
-//   P   = exp2(c (S s_k - m))    m moves only when it is 2^8 behind (as in the prompt kernel)
+//   P   = exp2(c (S s_k - m) + 11)    m moves only when it is 2^4 behind
 //   O^T[dims x heads] += s_v (V^T P)
 // The cache is read once, straight into the registers that hold the A operands:
 // the contraction of Q K^T runs over dims in the order in which 16-byte pieces of
@@ -196,6 +196,10 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 // keys by permutes, so no shared memory and no barrier stands between HBM and
 // the tensor cores.  e4m3 converts to fp16 exactly; bf16 queries are brought to
 // fp16 by a power of two per head (their largest value to [2^14, 2^15)).
+// P is rounded to fp16 (V's codes convert to it exactly), l sums it before.  The factor 2^11,
+// which O and l share, puts P <= 2^15 at the top of fp16's range: a weight down to 2^-25
+// of its warp's largest is rounded relative to itself, a smaller one to 2^-36 of it.  (Without
+// it the keys behind one that leads them by 18 and has V = 0 counted for nothing.)
 // A warp takes 32 keys at a time and keeps the next 32 keys' K and V in flight.
 // The context is shared out in one of these ways:
 //   clusters  a cluster of CTAs takes one (row, K/V head) and joins its parts
@@ -208,6 +212,7 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 //             they are many)
 constexpr int kAtWarps = 4;
 constexpr int kAtKeys = 32;  // keys per warp and step
+constexpr float kAtLead = 4.f, kAtBias = 11.f;  // log2 of how far m may fall behind; of what P is multiplied by
 
 // CTAs that an SM holds, by their registers.
 constexpr int kv8_per_sm(int ng, int D) { return ng == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2); }
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
                         else
                             x0 = fmaxf(x0, s[n][i][e]);
                     }
-                move |= x0 - m0[n] > 8.f || x1 - m1[n] > 8.f;
+                move |= x0 - m0[n] > kAtLead || x1 - m1[n] > kAtLead;
                 if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) {
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
                         o[n][i][3] *= r1;
                     }
                 }
-                const float b0 = m0[n] == -INFINITY ? 0.f : m0[n], b1 = m1[n] == -INFINITY ? 0.f : m1[n];
+                const float b0 = m0[n] == -INFINITY ? 0.f : m0[n] - kAtBias, b1 = m1[n] == -INFINITY ? 0.f : m1[n] - kAtBias;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
