@@ -71,3 +71,30 @@ def test_decode_keeps_the_weights_behind_a_sink(dev, lens, heads, kv, hd, dt, ws
             for h in range(a * heads // kv, (a + 1) * heads // kv):
                 want[r, h], tol[r, h] = attend(c["q"][r].reshape(heads, hd)[h], *kv_values, dt)
     near(run_decode(dev, c, max(lens), ws), want.reshape(len(lens), -1), tol.reshape(len(lens), -1))
+
+
+def huge_scores(n, hd, score):
+    """Keys whose scores are `score`, and minus it for the odd ones, for a query of 2^10 throughout; key 5 leads with half as much again."""
+    k = np.zeros((n, hd))
+    k[:, 0] = score * math.sqrt(hd) / 2.0 ** 10
+    k[1::2, 0] *= -1
+    k[5, 0] *= -1.5
+    return k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", [3e5, 1e7, 3e7, 6e7, 9e7])
+@pytest.mark.parametrize("heads,kv,hd,dt", [(16, 4, 64, wk.F16), (32, 2, 128, wk.BF16)])
+def test_decode_scores_of_any_size(dev, score, heads, kv, hd, dt):
+    """One key leads the others by millions: its V comes out."""
+    c = ops.make_decode([400, 130], heads, kv, hd, dt, seed=5)
+    k = huge_scores(401, hd, score)
+    c["scales"][0][:] = 2.0 ** math.ceil(math.log2(np.abs(k).max() / 448))
+    c["q"] = rounded(np.full(c["q"].shape, 2.0 ** 10), dt)
+    codes = e4m3_codes(k / c["scales"][0][0, 0])
+    for r, n in enumerate([401, 131]):
+        for j, page in enumerate(c["table"][r, : -(-n // PAGE)]):
+            part = codes[j * PAGE:min((j + 1) * PAGE, n)]
+            c["codes"][0][page, :, : len(part)] = part
+    want, tol = ops.ref_decode(c)
+    ops.close(run_decode(dev, c, 401, ws=True), want, tol)

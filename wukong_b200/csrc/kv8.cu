@@ -590,7 +590,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
                         o[n][i][3] *= r1;
                     }
                 }
-                const float b0 = m0[n] == -INFINITY ? 0.f : m0[n] - kAtBias, b1 = m1[n] == -INFINITY ? 0.f : m1[n] - kAtBias;
+                // (rounded up, so that P <= 2^15 holds for scores of any size)
+                const float b0 = m0[n] == -INFINITY ? 0.f : __fsub_ru(m0[n], kAtBias);
+                const float b1 = m1[n] == -INFINITY ? 0.f : __fsub_ru(m1[n], kAtBias);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
