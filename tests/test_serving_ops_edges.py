@@ -2,10 +2,10 @@
 
 Tolerances.  As in the other file, with what it leaves out: a softmax weight is
 multiplied with V in 16 bits, and in fp16 it is exact to half of 2^-24 at the
-least.  The kernels keep weights of one key that leads its row near 2^11 or
-above, so that this is at most 2^-36 of such a key's weight, and the weights sum
-to at least that of one: 2^-36 sum |v| of the keys that a row sees.  An output in
-fp16 is exact to 2^-25 at the least.
+least.  The kernels multiply the weights by 2^9 or more, relative to a score that
+some key of the row reaches, so that this is at most 2^-34 of that key's weight,
+and the weights sum to at least one such: 2^-34 sum |v| of the keys that a row
+sees.  An output in fp16 is exact to 2^-25 at the least.
 """
 import math
 
@@ -14,7 +14,7 @@ import pytest
 
 import wukong_b200 as wk
 from tests import test_serving_ops as ops
-from tests.test_serving_ops import CODES, PAGE, UNIT, e4m3_codes, rounded, run_decode
+from tests.test_serving_ops import CODES, PAGE, UNIT, e4m3_codes, rounded, run_decode, run_packed
 
 
 def attend(q, k, v, dt):
@@ -27,7 +27,7 @@ def attend(q, k, v, dt):
     S = (np.abs(k) @ np.abs(q)).max() / math.sqrt(d)
     u = UNIT[dt]
     tol = u * np.abs(o) + A * (u + 2 * (d * 2.0 ** -24 * S + 2.0 ** -20) + n * 2.0 ** -24) * (1 + u)
-    return o, tol + 2.0 ** -36 * np.abs(v).sum(0) + (2.0 ** -25 if dt == wk.F16 else 0.0)
+    return o, tol + 2.0 ** -34 * np.abs(v).sum(0) + (2.0 ** -25 if dt == wk.F16 else 0.0)
 
 
 def near(got, want, tol):
@@ -98,3 +98,55 @@ def test_decode_scores_of_any_size(dev, score, heads, kv, hd, dt):
             c["codes"][0][page, :, : len(part)] = part
     want, tol = ops.ref_decode(c)
     ops.close(run_decode(dev, c, 401, ws=True), want, tol)
+
+
+def packed_with_sinks(ql, kl, heads, kv, hd, dt, gap, seed):
+    rng = np.random.default_rng(seed)
+    c = ops.make_packed(ql, kl, heads, kv, hd, dt, seed)
+    c["q"] = rounded(np.full(c["q"].shape, gap / math.sqrt(hd)), dt)
+    for i in range(len(kl)):
+        for a in range(kv):
+            at = slice(c["ks"][i], c["ks"][i + 1]), slice(a * hd, (a + 1) * hd)
+            c["k"][at], c["v"][at] = (rounded(x, dt) for x in sinks(rng, kl[i], hd, gap, 200))
+    want, tol = np.zeros(c["q"].shape), np.zeros(c["q"].shape)
+    for i in range(len(ql)):
+        for h in range(heads):
+            a = h * kv // heads
+            k, v = (c[x][c["ks"][i]:c["ks"][i + 1], a * hd:(a + 1) * hd] for x in "kv")
+            for j in range(ql[i]):
+                n, at = kl[i] - ql[i] + j + 1, (c["qs"][i] + j, slice(h * hd, (h + 1) * hd))
+                want[at], tol[at] = attend(c["q"][at], k[:n], v[:n], dt)
+    return c, want, tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [12.0, 15.0, 18.0])
+@pytest.mark.parametrize("ql,kl,heads,kv,hd,dt", [
+    ([300], [700], 4, 2, 128, wk.F16),
+    ([400, 90], [400, 500], 2, 1, 64, wk.F16),
+    ([60], [2600], 2, 1, 128, wk.F16),              # a cluster shares the keys
+    ([300], [700], 4, 2, 128, wk.BF16),
+    ([50, 90], [60, 90], 6, 2, 64, wk.F16),         # the kernel of short sequences
+])
+def test_packed_keeps_the_weights_behind_a_sink(dev, ql, kl, heads, kv, hd, dt, gap):
+    c, want, tol = packed_with_sinks(ql, kl, heads, kv, hd, dt, gap, seed=int(gap) + heads)
+    near(run_packed(dev, c), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", [3e5, 1e7, 3e7, 6e7, 9e7])
+@pytest.mark.parametrize("ql,kl,heads,kv,hd,dt", [
+    ([300], [700], 4, 2, 128, wk.F16),
+    ([40], [2600], 2, 1, 64, wk.F16),
+    ([50, 90], [60, 90], 6, 2, 64, wk.F16),
+    ([50, 90], [60, 90], 6, 2, 128, wk.BF16),
+    ([300], [400], 4, 4, 64, wk.BF16),
+])
+def test_packed_scores_of_any_size(dev, ql, kl, heads, kv, hd, dt, score):
+    c = ops.make_packed(ql, kl, heads, kv, hd, dt, seed=3)
+    c["q"] = rounded(np.full(c["q"].shape, 2.0 ** 10), dt)
+    for i, n in enumerate(kl):
+        one = huge_scores(n, hd, score)[:, :1] / hd
+        c["k"][c["ks"][i]:c["ks"][i + 1]] = rounded(np.repeat(one, kv * hd, 1), dt)
+    want, tol = ops.ref_packed(c)
+    ops.close(run_packed(dev, c), want, tol)

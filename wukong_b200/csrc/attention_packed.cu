@@ -27,6 +27,20 @@ struct PackedArgs {
     bool out4;  // out's rows are 4-byte aligned
 };
 
+// Softmax weights are multiplied with V in V's type.  fp16 is exact to 2^-25 at the least, so
+// its weights go in as 2^bias p, at the top of its range: O and the sum l share the factor.
+// `lead`: log2 of how far the reference of p may fall behind the largest score (p <= 2^lead).
+// With bias 0 the keys behind one that leads them by 18 and has V = 0 counted for nothing; with
+// 9 a p down to 2^-23 is rounded relative to itself, a smaller one to 2^-34.  (24 prompts of
+// 1 to 1500 tokens, 16 / 4 heads of 64: 39.6 us, as with a lead of 8; 1 % more with 5, 8 % with 4.)
+// References are rounded up, so that 2^(lead + bias) bounds the weights for scores up to 10^8.
+template <typename T> struct PkWeight {
+    static constexpr float lead = 6.f, bias = 9.f;
+};
+template <> struct PkWeight<__nv_bfloat16> {
+    static constexpr float lead = 8.f, bias = 0.f;
+};
+
 // One CTA per (query row, head), 128 threads: a thread scores one key of each
 // block of 128, then owns one dimension of the output.
 template <typename T, int D>
@@ -89,12 +103,11 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // A CTA takes 64 rows of one sequence and K/V head, a row being a position and one
 // of the G heads of the group (heads inner, so no row is empty but at a sequence's end);
 // a warp takes 16 of them, with S, P and O in mma.sync fragments:
-//   S = Q K^T     P = exp2(c (S - m) + 8)     O += P V     l += row sums of P before rounding
+//   S = Q K^T     P = exp2(c (S - m) + b)     O += P V     l += row sums of P before rounding
 // Blocks of 64 keys come through two stages of cp.async.  The contraction of Q K^T runs
 // over dims in the order in which 16-byte pieces of a row fall to the four lanes
 // of a row group, so Q goes from global memory straight into its fragments and a K
-// fragment is one 16-byte read.  P in [0, 2^8] keeps the type's full precision down to
-// 2^-22 of the row's largest p in fp16.
+// fragment is one 16-byte read.  m is the running maximum itself, so b = 15 leaves P in fp16's range.
 // Latency bounds it: unit -> Q, K, V -> S -> softmax -> O.  Small CTAs, several to an SM, and
 // no tensor memory, barriers or maps to set up are what it has over the tcgen05 kernel: 100
 // sequences of 40 tokens, 16 / 4 heads of 64, take 10.5 us instead of 22.0.  A further block
@@ -268,7 +281,7 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float f = mx == m[i] ? 1.f : pk_ex2((m[i] - mx) * c2);
-                const float ref = mx == -INFINITY ? 0.f : mx * c2 - 8.f;
+                const float ref = mx == -INFINITY ? 0.f : __fmaf_ru(mx, c2, -PkWeight<T>::lead - PkWeight<T>::bias);
                 m[i] = mx;
                 l[i] *= f;
 #pragma unroll
@@ -369,13 +382,13 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
 // A CTA takes one unit: 2 tiles of 128 query rows of one K/V head, a tile being
 // PT = 128 / G positions times the G heads of the group (heads inner), so that a
 // K/V tile loaded once serves all of them.  Per block of 128 keys and tile t:
-//   S_t = Q_t K^T  (TMEM, fp32)       P_t = exp2(c (S_t - m))  (16 bits, over S_t in TMEM)
+//   S_t = Q_t K^T  (TMEM, fp32)       P_t = exp2(c (S_t - m) + b)  (16 bits, over S_t in TMEM)
 //   O_t += P_t V   (TMEM, fp32)       l_t += row sums of P_t before rounding
 // P is rounded to V's type, which is what the tensor cores multiply V with: at most
 // half a step of that type relative to each p, and l_t does not inherit it.
 // m is a maximum that is moved, and O_t and l_t scaled, only when it falls more
-// than 2^8 behind the running maximum: p <= 2^8 keeps its relative rounding, and
-// nearly every block skips the pass over O_t.  The first half of a block's
+// than 2^6 (bf16: 2^8) behind the running maximum, so that nearly every block
+// skips the pass over O_t.  The first half of a block's
 // exponentials is computed against the old maximum before the block's own is
 // known, and thrown away in the rare case that it moves.
 //   warps 0-3, 4-7   softmax of tile 0, tile 1 (one thread per row), epilogue
@@ -590,7 +603,7 @@ struct PkArgs {
     const int *q_starts, *k_starts;
     int n, q_rows, k_rows, G, GT, chunks;  // heads per K/V head, heads per tile, tiles of heads per K/V head
     int PT;                                // positions per tile
-    float scale_log2;
+    float scale_log2, shift;               // shift: the bias of P in units of the scores
     int vec;  // out is 16-byte aligned and strided
     int split;  // CTAs of a cluster, which share a unit's keys
     int *err;
@@ -942,7 +955,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             const int lim0 = shift + j0 + t * PT;     // of the tile's first row
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;
             const uint32_t s_t = tmem + t * 128 + lanes, o_t = tmem + 256 + t * 128 + lanes;
-            float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to
+            float m = -INFINITY, l = 0.f;  // m: what P is relative to, a maximum less the shift for its bias
             for (int j = 0; j < nt; ++j) {
                 // (the warp leaves as one: what follows is warp-wide)
                 if (!__all_sync(0xffffffffu, pk_wait(&B->s_full[t], j & 1, a.err, 57))) {
@@ -972,7 +985,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(sv[e]);
                 auto half = [&](int c, bool find, float m, f32x2(&sum)[2], uint32_t(&pv)[32]) {
-                    const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                    const float base = m == -INFINITY ? 0.f : __fmul_rd(-m, a.scale_log2);
                     const f32x2 base2 = pk_pair(base, base);
                     sum[0] = sum[1] = 0;
 #pragma unroll
@@ -999,12 +1012,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 if (j == 0) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(sv[i]));
+                    m = __fsub_ru(m, a.shift);
                 }
                 half(0, true, m, sum, pv);
                 const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                const bool move = (mb - m) * a.scale_log2 > 8.f || (m == -INFINITY && mb > m);
+                const bool move = (mb - m) * a.scale_log2 > PkWeight<T>::lead + PkWeight<T>::bias || (m == -INFINITY && mb > m);
                 if (__any_sync(0xffffffffu, move)) {
-                    const float mn = move ? mb : m;
+                    const float mn = move ? __fsub_ru(mb, a.shift) : m;
                     const float f = mn == m || m == -INFINITY ? 1.f : pk_ex2((m - mn) * a.scale_log2);
                     m = mn;
                     l *= f;
@@ -1209,6 +1223,7 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     a.chunks = (a.G + GT - 1) / GT;
     a.PT = 128 / GT;
     a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.shift = PkWeight<T>::bias / a.scale_log2;
     a.vec = ((uintptr_t)p.out % 16) == 0 && p.out_rs % 8 == 0;
     a.err = g_rt.d_error;
     const int PT = 128 / GT;
