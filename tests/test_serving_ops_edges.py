@@ -150,3 +150,29 @@ def test_packed_scores_of_any_size(dev, ql, kl, heads, kv, hd, dt, score):
         c["k"][c["ks"][i]:c["ks"][i + 1]] = rounded(np.repeat(one, kv * hd, 1), dt)
     want, tol = ops.ref_packed(c)
     ops.close(run_packed(dev, c), want, tol)
+
+
+# bf16 holds values up to 2^128: a mean of such values is one too, and the sum on the way to it must not pass fp32's range
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [127, 120, 0, -90, -100])
+@pytest.mark.parametrize("ql,kl,heads,kv,hd,extra,shift", [
+    ([300], [700], 4, 2, 128, 0, 0),
+    ([40], [2600], 2, 1, 64, 0, 0),
+    ([50, 90], [60, 90], 6, 2, 64, 0, 0),
+    ([50, 90], [60, 90], 6, 2, 128, 0, 0),
+    ([9, 40], [60, 40], 2, 1, 128, 3, 1),
+])
+def test_packed_values_of_any_size(dev, ql, kl, heads, kv, hd, extra, shift, power):
+    c = ops.make_packed(ql, kl, heads, kv, hd, wk.BF16, seed=4)
+    rng = np.random.default_rng(4)
+    c["v"] = rounded(rng.uniform(0.5, 1.0, c["v"].shape), wk.BF16) * 2.0 ** power
+    want, tol = np.zeros(c["q"].shape), np.zeros(c["q"].shape)
+    for i in range(len(ql)):
+        for h in range(heads):
+            a = h * kv // heads
+            k, v = (c[x][c["ks"][i]:c["ks"][i + 1], a * hd:(a + 1) * hd] for x in "kv")
+            for j in range(ql[i]):
+                n, at = kl[i] - ql[i] + j + 1, (c["qs"][i] + j, slice(h * hd, (h + 1) * hd))
+                want[at], tol[at] = attend(c["q"][at], k[:n], v[:n], wk.BF16)
+    near(run_packed(dev, c, extra, shift), want, tol)

@@ -37,8 +37,9 @@ struct PackedArgs {
 template <typename T> struct PkWeight {
     static constexpr float lead = 6.f, bias = 9.f;
 };
+// bf16 has fp32's range: 2^bias keeps the sums over up to 2^24 keys below V's own largest value.
 template <> struct PkWeight<__nv_bfloat16> {
-    static constexpr float lead = 8.f, bias = 0.f;
+    static constexpr float lead = 8.f, bias = -32.f;
 };
 
 // One CTA per (query row, head), 128 threads: a thread scores one key of each
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
         if (lane == 0) s_w[wid] = bm;
         __syncthreads();
         const float mn = fmaxf(m, fmaxf(fmaxf(s_w[0], s_w[1]), fmaxf(s_w[2], s_w[3])));
-        const float p = s == -INFINITY ? 0.f : expf(s - mn);
+        const float p = s == -INFINITY ? 0.f : expf(s - mn) * 0x1p-24f;  // (sums stay below V's largest value)
         s_p[tid] = p;
         __syncthreads();
         const float sum = warp_sum(p);
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // Blocks of 64 keys come through two stages of cp.async.  The contraction of Q K^T runs
 // over dims in the order in which 16-byte pieces of a row fall to the four lanes
 // of a row group, so Q goes from global memory straight into its fragments and a K
-// fragment is one 16-byte read.  m is the running maximum itself, so b = 15 leaves P in fp16's range.
+// fragment is one 16-byte read.  m is the running maximum itself, so b = lead + bias: 15 in fp16, -24 in bf16.
 // Latency bounds it: unit -> Q, K, V -> S -> softmax -> O.  Small CTAs, several to an SM, and
 // no tensor memory, barriers or maps to set up are what it has over the tcgen05 kernel: 100
 // sequences of 40 tokens, 16 / 4 heads of 64, take 10.5 us instead of 22.0.  A further block
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
             for (int c = 0; c < NC; ++c) dot += to_float(qr[lane + 32 * c]) * to_float(kp[j * a.k_rs + lane + 32 * c]);
             dot = warp_sum(dot) * c2;
             const float mn = fmaxf(mr, dot), f = mr == mn ? 1.f : pk_ex2(mr - mn);
-            const float w = dot == -INFINITY ? 0.f : pk_ex2(dot - mn);
+            const float w = dot == -INFINITY ? 0.f : pk_ex2(dot - mn + (PkWeight<T>::lead + PkWeight<T>::bias));
             mr = mn;
             lr = lr * f + w;
 #pragma unroll
