@@ -176,3 +176,29 @@ def test_packed_values_of_any_size(dev, ql, kl, heads, kv, hd, extra, shift, pow
                 n, at = kl[i] - ql[i] + j + 1, (c["qs"][i] + j, slice(h * hd, (h + 1) * hd))
                 want[at], tol[at] = attend(c["q"][at], k[:n], v[:n], wk.BF16)
     near(run_packed(dev, c, extra, shift), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [119, 100, 0, -90, -100])
+@pytest.mark.parametrize("lens,heads,kv,hd,ws", [
+    ([777], 16, 4, 64, True),
+    ([300, 5, 1, 450, 333] * 6, 16, 8, 128, False),
+    ([40, 2000, 130, 700] * 8, 32, 2, 128, True),
+    ([9000], 8, 1, 128, True),
+])
+def test_decode_values_of_any_size(dev, lens, heads, kv, hd, ws, power):
+    """Page scales from the least to the largest that bf16 rows give, codes up to 448."""
+    c = ops.make_decode([n - 1 for n in lens], heads, kv, hd, wk.BF16, seed=6)
+    rng = np.random.default_rng(6)
+    values = np.where(c["codes"][1] == 0x7F, np.nan, rng.uniform(200.0, 448.0, c["codes"][1].shape))
+    c["codes"][1] = e4m3_codes(values)
+    c["scales"][1] = np.where(np.isnan(c["scales"][1]), np.nan, 2.0 ** power)
+    want, tol = np.zeros((len(lens), heads, hd)), np.zeros((len(lens), heads, hd))
+    for r, n in enumerate(lens):
+        pages = c["table"][r, : -(-n // PAGE)]
+        for a in range(kv):
+            k, v = ((CODES[c["codes"][x][pages, a]] * c["scales"][x][pages, a][:, None, None]).reshape(-1, hd)[:n]
+                    for x in range(2))
+            for h in range(a * heads // kv, (a + 1) * heads // kv):
+                want[r, h], tol[r, h] = attend(c["q"][r].reshape(heads, hd)[h], k, v, wk.BF16)
+    near(run_decode(dev, c, max(lens), ws), want.reshape(len(lens), -1), tol.reshape(len(lens), -1))

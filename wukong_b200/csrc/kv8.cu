@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 // P is rounded to fp16 (V's codes convert to it exactly), l sums it before.  The factor 2^11,
 // which O and l share, puts P <= 2^15 at the top of fp16's range: a weight down to 2^-25
 // of its warp's largest is rounded relative to itself, a smaller one to 2^-36 of it.  (Without
-// it the keys behind one that leads them by 18 and has V = 0 counted for nothing.)
+// it the keys behind one that leads them by 18 and has V = 0 counted for nothing.)  O and l
+// carry 2^-40 besides, so that no sum passes V's own largest value, which in bf16 is fp32's.
 // A warp takes 32 keys at a time and keeps the next 32 keys' K and V in flight.
 // The context is shared out in one of these ways:
 //   clusters  a cluster of CTAs takes one (row, K/V head) and joins its parts
@@ -213,6 +214,7 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 constexpr int kAtWarps = 4;
 constexpr int kAtKeys = 32;  // keys per warp and step
 constexpr float kAtLead = 4.f, kAtBias = 11.f;  // log2 of how far m may fall behind; of what P is multiplied by
+constexpr float kAtSum = 0x1p-40f;              // O and l over P V and P
 
 // CTAs that an SM holds, by their registers.
 constexpr int kv8_per_sm(int ng, int D) { return ng == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2); }
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
     }
     for (int u = u0; u < u1; u += step) {
         const int cur = page;
-        const float cks = ks, cvs = vs;
+        const float cks = ks, cvs = vs * kAtSum;
         page = next_page;
         next_page = page_of(u + 2 * step);
         if (page >= 0) {
@@ -665,6 +667,8 @@ __global__ void __launch_bounds__(kAtWarps * 32, kv8_per_sm(NG, D)) kv8_attn_ker
             l0[n] += __shfl_xor_sync(0xffffffffu, l0[n], d);
             l1[n] += __shfl_xor_sync(0xffffffffu, l1[n], d);
         }
+        l0[n] *= kAtSum;
+        l1[n] *= kAtSum;
         const int h = n * 8 + 2 * t;
         if (g == 0) {
             s_m[warp][h] = m0[n];
