@@ -14,6 +14,7 @@ import pytest
 
 import wukong_b200 as wk
 from tests import test_serving_ops as ops
+from tests.gpu_util import alloc, down, free, up
 from tests.test_serving_ops import CODES, PAGE, UNIT, e4m3_codes, rounded, run_decode, run_packed
 
 
@@ -202,3 +203,21 @@ def test_decode_values_of_any_size(dev, lens, heads, kv, hd, ws, power):
             for h in range(a * heads // kv, (a + 1) * heads // kv):
                 want[r, h], tol[r, h] = attend(c["q"][r].reshape(heads, hd)[h], k, v, wk.BF16)
     near(run_decode(dev, c, max(lens), ws), want.reshape(len(lens), -1), tol.reshape(len(lens), -1))
+
+
+@pytest.mark.gpu
+def test_plan_with_the_largest_row_capacity(dev):
+    """2^31 - 1 rows of room, which no step in 32 bits may leave."""
+    cap = 2 ** 31 - 1
+    ctx, add, table = np.array([70, 0]), np.array([2, 130]), np.array([[4, 3, -1, -1], [-1, -1, -1, -1]])
+    want = ops.ref_plan(ctx, add, table, np.array([7, 8, 9]), 3, 140)
+    b = [up(np.asarray(x, np.int32)) for x in (np.zeros(3), np.zeros(2), table, np.zeros(3), ctx, add, [7, 8, 9], [3])]
+    starts, lens, tab, status, pctx, padd, pages, n_free = b
+    seq, pos = alloc(4 * cap), alloc(4 * cap)
+    wk.check(dev.wk_batch_plan(starts, lens, seq, pos, None, cap, tab, 4, status, pctx, padd, 2, pages, n_free, 3))
+    for p, name in ((seq, "row_seq"), (pos, "row_pos")):
+        assert np.array_equal(down(p, 140, np.int32), want[name])
+        assert (down(p + 4 * (cap - 100000), 100000, np.int32) == -1).all()
+    assert np.array_equal(down(tab, (2, 4), np.int32), want["table"])
+    assert np.array_equal(down(status, 3, np.int32), want["status"])
+    free(*b, seq, pos)

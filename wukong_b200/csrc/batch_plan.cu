@@ -118,9 +118,11 @@ __global__ void __launch_bounds__(kPlanThreads) batch_plan_kernel(PlanArgs a) {
     }
     __syncthreads();
     const int total = s_start[a.n], taken = s_base[a.n];
-    const int g0 = blockIdx.x * kPlanThreads + tid, gn = gridDim.x * kPlanThreads;
+    // (unsigned: rows_cap and the new pages reach 2^31 - 1, and a step beyond them must not come out negative)
+    const unsigned g0 = blockIdx.x * kPlanThreads + tid, gn = gridDim.x * kPlanThreads;
     // rows
-    for (int r = g0; r < a.rows_cap; r += gn) {
+    for (unsigned x = g0; x < (unsigned)a.rows_cap; x += gn) {
+        const int r = (int)x;
         int seq = -1, pos = -1;
         long long slot = -1;
         if (r < total) {
@@ -145,12 +147,13 @@ __global__ void __launch_bounds__(kPlanThreads) batch_plan_kernel(PlanArgs a) {
         if (a.row_slot) a.row_slot[r] = slot;
     }
     // new table entries
-    for (int j = g0; j < taken; j += gn) {
+    for (unsigned x = g0; x < (unsigned)taken; x += gn) {
+        const int j = (int)x;
         const int seq = last_le(s_base, a.n, j);
         a.table[(long)seq * a.max_pages + pages(s_ctx[seq]) + (j - s_base[seq])] = j < n_free ? a.free_pages[j] : -1;
     }
     // per sequence
-    for (int i = g0; i < a.n; i += gn) {
+    for (unsigned i = g0; i < (unsigned)a.n; i += gn) {
         a.starts[i] = s_start[i];
         a.lens[i] = sat((long long)s_ctx[i] + s_add[i]);
     }
@@ -199,7 +202,7 @@ int wk_batch_plan(int *starts, int *lens, int *row_seq, int *row_pos, long long 
     }
     // one thread per row (or sequence), at most one CTA per SM
     const int work = rows_cap > n ? rows_cap : n;
-    int ctas = (work + kPlanThreads - 1) / kPlanThreads;
+    int ctas = (work - 1) / kPlanThreads + 1;
     if (ctas > g_rt.num_sms) ctas = g_rt.num_sms;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
