@@ -177,7 +177,8 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
  * q_starts[i] .. q_starts[i+1] - 1 and the key rows k_starts[i] .. k_starts[i+1] - 1
  * (device int [n + 1], ascending), and its queries are the last of its keys: query j
  * of Lq sees keys 0 .. Lk - Lq + j of its own sequence; one that sees none gets
- * zeros.  Rows outside every sequence are neither read nor written.  q / out
+ * zeros.  Starts beyond q_rows or k_rows count as q_rows or k_rows (a plan of more
+ * rows than there is room for).  Rows outside every sequence are neither read nor written.  q / out
  * [q_rows][n_heads][head_dim], k / v [k_rows][kv_heads][head_dim] with row strides in
  * elements (the slices of fused q|k|v rows serve; q, k and v 16-byte aligned with
  * strides that are multiples of 8 take the tensor-core kernel, others a slow one);

@@ -15,7 +15,7 @@ import pytest
 import wukong_b200 as wk
 from tests import test_serving_ops as ops
 from tests.gpu_util import alloc, down, free, up
-from tests.test_serving_ops import CODES, PAGE, UNIT, e4m3_codes, rounded, run_decode, run_packed
+from tests.test_serving_ops import CODES, PAGE, UNIT, e4m3_codes, rounded, run_decode, run_packed, to_bits
 
 
 def attend(q, k, v, dt):
@@ -221,3 +221,27 @@ def test_plan_with_the_largest_row_capacity(dev):
     assert np.array_equal(down(tab, (2, 4), np.int32), want["table"])
     assert np.array_equal(down(status, 3, np.int32), want["status"])
     free(*b, seq, pos)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,extra", [(64, 0), (64, 1), (128, 0), (128, 1)])
+@pytest.mark.parametrize("lens,room", [([30, 50, 20], 61), ([30, 50, 20], 30), ([400, 300], 550)])
+def test_packed_prompts_with_less_room_than_rows(dev, lens, room, hd, extra):
+    """Starts of a plan that go beyond the rows: the rows that there are come out as their sequence gives them."""
+    c = ops.make_packed(lens, lens, 4, 2, hd, wk.F16, seed=9)
+    cut = dict(c, q=c["q"][:room], k=c["k"][:room], v=c["v"][:room], qs=np.minimum(c["qs"], room), ks=np.minimum(c["ks"], room))
+    want, tol = ops.ref_packed(cut)
+
+    def laid(x):
+        full = np.full((room, x.shape[1] + extra), np.nan)
+        full[:, : x.shape[1]] = x
+        return up(to_bits(full, wk.F16))
+    q, k, v = (laid(cut[x]) for x in "qkv")
+    starts, w = up(c["qs"].astype(np.int32)), 4 * hd
+    out = up(np.full((room + 9) * w, 0x3555, np.uint16))
+    wk.check(dev.wk_attention_packed(out, w, q, w + extra, k, 2 * hd + extra, v, 2 * hd + extra, starts, starts, len(lens),
+                                     room, room, 4, 2, hd, wk.F16))
+    got = down(out, (room + 9, w), np.uint16)
+    free(q, k, v, starts, out)
+    assert (got[room:] == 0x3555).all()
+    ops.close(got[:room].view(np.float16).astype(np.float64), want, tol)

@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
     const int kh = h / (a.heads / a.kv_heads);
     pdl_wait();
     pdl_trigger();
-    // the sequence that holds this row (starts ascend; an empty sequence holds none)
+    // the sequence that holds this row (starts ascend; an empty sequence holds none); starts beyond the
+    // rows count as the end of them, as in the other kernels
     if (tid == 0) s_seq[0] = -1;
     __syncthreads();
     for (int i = tid; i < a.n; i += 128)
@@ -61,7 +62,7 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
     __syncthreads();
     const int seq = s_seq[0];
     if (seq < 0) return;
-    const int q0 = a.q_starts[seq], ql = a.q_starts[seq + 1] - q0;
+    const int q0 = max(a.q_starts[seq], 0), ql = min(a.q_starts[seq + 1], a.q_rows) - q0;
     const int k0 = min(max(a.k_starts[seq], 0), a.k_rows);
     const int kl = min(max(a.k_starts[seq + 1], k0), a.k_rows) - k0;
     const int len = min(kl, kl - ql + (row - q0) + 1);
