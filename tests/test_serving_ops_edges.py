@@ -245,3 +245,16 @@ def test_packed_prompts_with_less_room_than_rows(dev, lens, room, hd, extra):
     free(q, k, v, starts, out)
     assert (got[room:] == 0x3555).all()
     ops.close(got[:room].view(np.float16).astype(np.float64), want, tol)
+
+
+def bits(x, dt):
+    return to_bits(x, dt).view(np.uint16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,heads,kv,hd,dt", [(512, 8, 1, 128, wk.F16), (760, 16, 4, 64, wk.BF16), (512, 32, 8, 128, wk.BF16)])
+def test_packed_prompt_too_short_for_a_cluster(dev, n, heads, kv, hd, dt):
+    """A prompt whose keys would not repay sharing them: the very results that it has among many, where CTAs are few enough."""
+    c = ops.make_packed([n] + [250] * 40, [n] + [250] * 40, heads, kv, hd, dt, seed=n)
+    alone = dict(c, qs=c["qs"][:2], ks=c["ks"][:2], **{x: c[x][:n] for x in "qkv"})
+    assert np.array_equal(bits(run_packed(dev, alone), dt), bits(run_packed(dev, c)[:n], dt))

@@ -405,8 +405,8 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
 // V behind the sequence's end to zero, and every infinity or NaN inside it too,
 // noting its key and dimension; rows that do see that key get NaN there.
 //
-// Where the units are fewer than half the SMs, a cluster of CTAs takes each, with
-// consecutive shares of its key blocks, and joins O, m and l through distributed
+// Where the units are fewer than half the SMs and their keys many, a cluster of CTAs takes
+// each, with consecutive shares of its key blocks, and joins O, m and l through distributed
 // shared memory.
 //
 // What bounds it: one block of two tiles takes 3200 to 3400 cycles with D = 128, of
@@ -1230,19 +1230,12 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     a.err = g_rt.d_error;
     const int PT = 128 / GT;
     // units: ceil(length / (2 PT)) per sequence
-    const long long most = (long long)p.q_rows / (2 * PT) + p.n;
+    const long long most = p.n == 1 ? (p.q_rows + 2ll * PT - 1) / (2 * PT) : (long long)p.q_rows / (2 * PT) + p.n;
     const long long units = most < p.q_rows ? most : p.q_rows;
     const long long ctas = units * p.kv_heads * a.chunks;
-    // Few units and long sequences: a cluster to each, with two blocks of keys or more per CTA
-    // (1 prompt of 2000 rows behind 14000, 8 heads over 1, 63 units: 225 us with a CTA each, 127 to
-    // 155 with two, as the clock allows).
-    long long split = g_rt.num_sms / ctas, blocks = p.k_rows / ((long long)kPkKeys * p.n);
-    if (split > blocks / 2) split = blocks / 2;
-    a.split = split < 2 ? 1 : split > 8 ? 8 : (int)split;
     const long long z = (units + kPkGridY - 1) / kPkGridY;
-    if ((long long)p.kv_heads * a.chunks * a.split > 0x7fffffffll || z > 65535) return cudaErrorInvalidConfiguration;
+    if ((long long)p.kv_heads * a.chunks * 8 > 0x7fffffffll || z > 65535) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.kv_heads * a.chunks * a.split, (unsigned)(units < kPkGridY ? units : kPkGridY), (unsigned)z);
     cfg.blockDim = dim3(kPkThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -1250,10 +1243,38 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = g_rt.pdl ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.split;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
+    // Few units and long sequences: a cluster to each, where all run at once and it saves more
+    // blocks of keys (of the mean length) than its join takes: 11 us with 2 or 3 CTAs, 8 us
+    // with more, heads of 64 7 and 5 us, 3 us where a unit has a row or two, a block taking 1.6.  8 heads of 128 over 1, us without / with
+    // 2 / 4 / 8 CTAs to a unit:
+    //   512 rows  13.8 / 21.7 / 16.5 / 30.0 (16 clusters of 8 do not fit)   500 behind 4000  67 / 48 / 30 / 40
+    //   1024      20.6 / 25.2 / 18.3 / -     2048  34.1 / 32.6 / - / -      2000 behind 14000  216 / 126 / - / -
+    static int at_once[9], at_once_on = -1;  // clusters of a size that run at once, on which device
+    if (at_once_on != g_rt.device) {
+        for (int c = 2; c <= 8; ++c) {
+            cfg.gridDim = dim3(c);
+            attr[1].val.clusterDim.x = c;
+            cfg.numAttrs = 2;
+            const cudaError_t e = cudaOccupancyMaxActiveClusters(&at_once[c], kern, &cfg);
+            if (e != cudaSuccess) return e;
+        }
+        at_once_on = g_rt.device;
+    }
+    const double blocks = (double)p.k_rows / ((double)kPkKeys * p.n);
+    long long split = blocks / 2 < g_rt.num_sms / ctas ? (long long)(blocks / 2) : g_rt.num_sms / ctas;
+    if (split > 8) split = 8;
+    // (of one sequence the units are exact; of several they are fewer than `units`, which leaves room)
+    while (p.n == 1 && split > 1 && at_once[split] < ctas) --split;
+    const double full = (double)p.q_rows / ((double)p.n * 2 * PT);  // how full units are, on average
+    const double join = 2 + (full < 1 ? full : 1) * ((D == 64 ? 1 : 3) + (split < 4 ? D / 64 : 0));  // in blocks
+    const double longer = p.n > 2 ? 1.5 : 1;  // of several, the longest ends last
+    if (blocks * longer * (split - 1) < split * join) split = 1;
+    a.split = split < 2 ? 1 : (int)split;
+    cfg.gridDim = dim3(p.kv_heads * a.chunks * a.split, (unsigned)(units < kPkGridY ? units : kPkGridY), (unsigned)z);
+    attr[1].val.clusterDim.x = a.split;
     cfg.numAttrs = a.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
