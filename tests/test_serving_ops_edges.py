@@ -258,3 +258,25 @@ def test_packed_prompt_too_short_for_a_cluster(dev, n, heads, kv, hd, dt):
     c = ops.make_packed([n] + [250] * 40, [n] + [250] * 40, heads, kv, hd, dt, seed=n)
     alone = dict(c, qs=c["qs"][:2], ks=c["ks"][:2], **{x: c[x][:n] for x in "qkv"})
     assert np.array_equal(bits(run_packed(dev, alone), dt), bits(run_packed(dev, c)[:n], dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [700, 2000])
+@pytest.mark.parametrize("heads,kv,hd,dt", [(16, 8, 128, wk.F16), (16, 16, 64, wk.BF16)])
+@pytest.mark.parametrize("others", [[0] * 63, [1] * 90, [5, 0, 40] * 20])
+def test_packed_long_prompt_among_idle_and_short_sequences(dev, n, heads, kv, hd, dt, others):
+    """Sequences without rows and short ones do not change how a long prompt is computed: its results are the very same."""
+    lens = others[: len(others) // 2] + [n] + others[len(others) // 2:]
+    c = ops.make_packed(lens, lens, heads, kv, hd, dt, seed=n)
+    i = len(others) // 2
+    at = slice(c["qs"][i], c["qs"][i + 1])
+    # alone: beside three of its like, so that CTAs are not few
+    like = dict(c, qs=np.arange(4) * n, ks=np.arange(4) * n, **{x: np.concatenate([c[x][at]] * 3) for x in "qkv"})
+    got = run_packed(dev, c)
+    assert np.array_equal(bits(got[at], dt), bits(run_packed(dev, like)[:n], dt))
+    rest = np.ones(len(got), bool)
+    rest[at] = False
+    short = dict(c, qs=np.concatenate([c["qs"][: i + 1], c["qs"][i + 2:] - n]),
+                 ks=np.concatenate([c["ks"][: i + 1], c["ks"][i + 2:] - n]), **{x: c[x][rest] for x in "qkv"})
+    want, tol = ops.ref_packed(short)
+    ops.close(got[rest], want, tol)

@@ -25,6 +25,8 @@ struct PackedArgs {
     int n, q_rows, k_rows, heads, kv_heads;
     float scale;
     bool out4;  // out's rows are 4-byte aligned
+    int reach;  // sequences of up to so many keys are the short kernel's, longer ones the tcgen05 kernel's
+    int longer; // how many longer ones there can be
 };
 
 // Softmax weights are multiplied with V in V's type.  fp16 is exact to 2^-25 at the least, so
@@ -113,8 +115,8 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // Latency bounds it: unit -> Q, K, V -> S -> softmax -> O.  Small CTAs, several to an SM, and
 // no tensor memory, barriers or maps to set up are what it has over the tcgen05 kernel: 100
 // sequences of 40 tokens, 16 / 4 heads of 64, take 10.5 us instead of 22.0.  A further block
-// of 64 keys costs 1.6 us with D = 128, so long sequences are not for it (where they begin
-// to cost more stands at the launch).
+// of 64 keys costs 1.6 us with D = 128, so sequences of more than `reach` keys are not for it
+// (where they begin to cost more stands at the launch).
 // A row whose result is not finite is computed again over the keys that it sees alone,
 // for a masked key has p = 0, and 0 * NaN is NaN.
 __device__ __forceinline__ float pk_ex2(float x) {
@@ -179,12 +181,12 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
         const int i = lo + tid, r0 = start(i), r1 = max(start(i + 1), r0), k0 = a.k_starts[i], k1 = a.k_starts[i + 1];
         const int k = unit - base(r0, i);
         if (k >= 0 && unit < base(r1, i + 1) && (long)k * 64 < (long)(r1 - r0) * G) {
-            s_unit[0] = 1;
             s_unit[1] = r0;
             s_unit[2] = r1 - r0;
             s_unit[3] = min(max(k0, 0), a.k_rows);
             s_unit[4] = min(max(k1, s_unit[3]), a.k_rows) - s_unit[3];
             s_unit[5] = k * 64;
+            s_unit[0] = s_unit[4] <= a.reach;
         }
     }
     __syncthreads();
@@ -608,6 +610,7 @@ struct PkArgs {
     float scale_log2, shift;               // shift: the bias of P in units of the scores
     int vec;  // out is 16-byte aligned and strided
     int split;  // CTAs of a cluster, which share a unit's keys
+    int reach;  // sequences of up to so many keys are left to the short kernel (-1: none)
     int *err;
 };
 
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             s.ql = min(max(q1, s.q0), a.q_rows) - s.q0;
             s.k0 = min(max(k0, 0), a.k_rows);
             s.kl = min(max(k1, s.k0), a.k_rows) - s.k0;
-            units = (s.ql + 2 * PT - 1) / (2 * PT);
+            units = s.kl > a.reach ? (s.ql + 2 * PT - 1) / (2 * PT) : 0;
         }
         return s;
     };
@@ -1227,10 +1230,12 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     a.scale_log2 = p.scale * 1.4426950408889634f;
     a.shift = PkWeight<T>::bias / a.scale_log2;
     a.vec = ((uintptr_t)p.out % 16) == 0 && p.out_rs % 8 == 0;
+    a.reach = p.reach;
     a.err = g_rt.d_error;
     const int PT = 128 / GT;
     // units: ceil(length / (2 PT)) per sequence
-    const long long most = p.n == 1 ? (p.q_rows + 2ll * PT - 1) / (2 * PT) : (long long)p.q_rows / (2 * PT) + p.n;
+    const int n = p.longer;  // that are this kernel's
+    const long long most = n == 1 ? (p.q_rows + 2ll * PT - 1) / (2 * PT) : (long long)p.q_rows / (2 * PT) + n;
     const long long units = most < p.q_rows ? most : p.q_rows;
     const long long ctas = units * p.kv_heads * a.chunks;
     const long long z = (units + kPkGridY - 1) / kPkGridY;
@@ -1263,14 +1268,14 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
         }
         at_once_on = g_rt.device;
     }
-    const double blocks = (double)p.k_rows / ((double)kPkKeys * p.n);
+    const double blocks = (double)p.k_rows / ((double)kPkKeys * n);
     long long split = blocks / 2 < g_rt.num_sms / ctas ? (long long)(blocks / 2) : g_rt.num_sms / ctas;
     if (split > 8) split = 8;
     // (of one sequence the units are exact; of several they are fewer than `units`, which leaves room)
-    while (p.n == 1 && split > 1 && at_once[split] < ctas) --split;
-    const double full = (double)p.q_rows / ((double)p.n * 2 * PT);  // how full units are, on average
+    while (n == 1 && split > 1 && at_once[split] < ctas) --split;
+    const double full = (double)p.q_rows / ((double)n * 2 * PT);  // how full units are, on average
     const double join = 2 + (full < 1 ? full : 1) * ((D == 64 ? 1 : 3) + (split < 4 ? D / 64 : 0));  // in blocks
-    const double longer = p.n > 2 ? 1.5 : 1;  // of several, the longest ends last
+    const double longer = n > 2 ? 1.5 : 1;  // of several, the longest ends last
     if (blocks * longer * (split - 1) < split * join) split = 1;
     a.split = split < 2 ? 1 : (int)split;
     cfg.gridDim = dim3(p.kv_heads * a.chunks * a.split, (unsigned)(units < kPkGridY ? units : kPkGridY), (unsigned)z);
@@ -1342,46 +1347,58 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
     if (g_rt.device < 0) return fail("wk_attention_packed: cuda_init() has not been called");
     DeviceGuard guard;
     PackedArgs a{out, out_rs, q, k, v, q_rs, k_rs, v_rs, q_starts, k_starts, n, q_rows, k_rows, n_heads, kv_heads,
-                 1.0f / sqrtf((float)head_dim), (uintptr_t)out % 4 == 0 && out_rs % 2 == 0};
+                 1.0f / sqrtf((float)head_dim), (uintptr_t)out % 4 == 0 && out_rs % 2 == 0, -1, n};
     cudaStream_t s = stream();
     cudaError_t e;
     // TMA wants 16-byte aligned bases and strides; what is not goes row by row
     const uintptr_t low = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v;
     if (low % 16 == 0 && (q_rs | k_rs | v_rs) % 8 == 0 && k_rows > 0) {
         const int G = n_heads / kv_heads, GT = G < 128 ? G : 128;
-        // Short sequences: by their mean length, which is all that is known here, with room for
-        // one that is much longer than the others where there are several.  us, this kernel / tcgen05,
-        // 32 / 8 heads of 128:
-        //   1 of 97           8.0 /  9.3     24 of 16        7.0 / 15.4    24 of 1 to 300 (mean 62)  24.3 / 24.5
-        //   1 of 200         10.1 / 10.4     24 of 73 to 97 23.6 / 26.6    24 of 1 to 500 (97)       42.1 / 32.8
-        //   100 of 16        14.4 / 44.6     400 of 40       129 / 218     6 of 1 to 300 (80)        16.2 / 12.6
+        // Short sequences go to the kernel for them.  The host knows room and count only, and idle
+        // sequences and room without rows hide a long one; so where all of them may be short but one
+        // could have more than `reach` keys, both kernels are launched and each takes its own sequences
+        // by their lengths.  A sequence by itself and short ones throughout, us, short kernel / tcgen05 /
+        // both, 32 / 8 heads of 128:
+        //   1 of 192           9.6 / 10.1         24 of 16     7.5 / 15.1 /  8.9    100 of 16  15.1 / 44.1 / 19.0
+        //   1 of 256          11.6 / 10.2         24 of 60    14.8 / 17.2 / 18.4    100 of 40  36.8 / 55.0 / 45.4
+        //   1 of 4096, 63 of 0  452 / 127 / 129   24 of 97    26.6 / 26.2           400 of 40   144 /  231 /  182
         // 16 / 4 heads of 64:
-        //   1 of 256          7.3 /  9.0     24 of 97        7.9 / 13.3    24 of 1 to 300 (62)       11.5 / 12.9
-        //   100 of 40        10.5 / 22.0     24 of 200      16.9 / 20.7    24 of 1 to 500 (97)       17.5 / 16.7
-        const long long shorter = (head_dim == 64 ? 112 : 64) * (n <= 2 ? 2 : 1);
+        //   1 of 384           9.5 / 10.2         24 of 40     5.6 /  7.4 /  7.6    100 of 40  11.7 / 22.7 / 15.7
+        //   1 of 768          17.3 / 16.8         24 of 97    10.1 / 14.0 / 13.4    400 of 97   109 /  175 /  150
+        //   1 of 4096, 63 of 0  134 /  59 /  61   24 of 200   16.9 / 20.7
+        const int reach = head_dim == 64 ? 512 : 256;
+        const int mean = head_dim == 64 ? 112 : 48;
         // base(n) of that kernel, with all rows
         long long units = (long long)q_rows * G / 64 + n;
         if (units > q_rows) units = q_rows;
-        if (G <= 64 && units <= 65535 && kv_heads <= 65535 && k_rows <= shorter * n) {
+        const bool some_short = G <= 64 && units <= 65535 && kv_heads <= 65535 &&
+                                (n == 1 ? k_rows <= reach * 3 / 4 : k_rows <= reach || k_rows <= (long long)mean * n);
+        const bool some_long = !some_short || k_rows > reach;
+        const int longer = k_rows / (reach + 1);  // key rows are nobody's twice
+        a.reach = some_short ? reach : -1;
+        a.longer = some_short && longer < n ? longer : n;
+        e = cudaSuccess;
+        if (some_long) {
+            PkMaps maps;
+            if (!pk_map(&maps.q, q, dtype, head_dim, n_heads, q_rows, q_rs, GT, 128 / GT) ||
+                !pk_map(&maps.k, k, dtype, head_dim, kv_heads, k_rows, k_rs, 1, kPkKeys) ||
+                !pk_map(&maps.v, v, dtype, head_dim, kv_heads, k_rows, v_rs, 1, kPkKeys))
+                return fail("wk_attention_packed: cuTensorMapEncodeTiled failed");
+            if (dtype == kF16)
+                e = head_dim == 64 ? launch_packed<__half, 64>(a, maps, GT, s)
+                                   : launch_packed<__half, 128>(a, maps, GT, s);
+            else
+                e = head_dim == 64 ? launch_packed<__nv_bfloat16, 64>(a, maps, GT, s)
+                                   : launch_packed<__nv_bfloat16, 128>(a, maps, GT, s);
+        }
+        if (some_short && e == cudaSuccess) {
             if (dtype == kF16)
                 e = head_dim == 64 ? launch_short<__half, 64>(a, (int)units, s)
                                    : launch_short<__half, 128>(a, (int)units, s);
             else
                 e = head_dim == 64 ? launch_short<__nv_bfloat16, 64>(a, (int)units, s)
                                    : launch_short<__nv_bfloat16, 128>(a, (int)units, s);
-            if (e != cudaSuccess) return fail_cuda("wk_attention_packed", e);
-            return 0;
         }
-        PkMaps maps;
-        if (!pk_map(&maps.q, q, dtype, head_dim, n_heads, q_rows, q_rs, GT, 128 / GT) ||
-            !pk_map(&maps.k, k, dtype, head_dim, kv_heads, k_rows, k_rs, 1, kPkKeys) ||
-            !pk_map(&maps.v, v, dtype, head_dim, kv_heads, k_rows, v_rs, 1, kPkKeys))
-            return fail("wk_attention_packed: cuTensorMapEncodeTiled failed");
-        if (dtype == kF16)
-            e = head_dim == 64 ? launch_packed<__half, 64>(a, maps, GT, s) : launch_packed<__half, 128>(a, maps, GT, s);
-        else
-            e = head_dim == 64 ? launch_packed<__nv_bfloat16, 64>(a, maps, GT, s)
-                               : launch_packed<__nv_bfloat16, 128>(a, maps, GT, s);
     } else if (dtype == kF16)
         e = head_dim == 64 ? launch_rows<__half, 64>(a, s) : launch_rows<__half, 128>(a, s);
     else
