@@ -280,3 +280,76 @@ def test_packed_long_prompt_among_idle_and_short_sequences(dev, n, heads, kv, hd
                  ks=np.concatenate([c["ks"][: i + 1], c["ks"][i + 2:] - n]), **{x: c[x][rest] for x in "qkv"})
     want, tol = ops.ref_packed(short)
     ops.close(got[rest], want, tol)
+
+
+# The tcgen05 kernel where sequences are many, far apart or beside others that are not finite: lengths
+# that send them to it.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,dt,keys", [(64, wk.F16, 130), (128, wk.BF16, 60)])
+def test_packed_many_sequences_behind_contexts_and_a_late_start(dev, hd, dt, keys):
+    """More sequences than one pass over their lengths takes; the first starts behind rows of nobody."""
+    rng = np.random.default_rng(5)
+    ql = rng.integers(0, 4, 900)
+    kl = ql + rng.integers(keys, keys + 9, 900)
+    c = ops.make_packed([7, *ql], [9, *kl], 4, 2, hd, dt, seed=17)
+    want, tol = ops.ref_packed(c)
+    d = dict(c, qs=c["qs"][1:], ks=c["ks"][1:])
+    got = run_packed(dev, d)
+    assert (bits(got[:7], dt) == 0x3555).all()  # not written
+    ops.close(got[7:], want[7:], tol[7:])
+    assert np.array_equal(got[7:], run_packed(dev, d)[7:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("hd,dt", [(64, wk.F16), (128, wk.F16), (64, wk.BF16)])
+def test_packed_longer_sequences_do_not_touch_each_other(dev, bad, hd, dt):
+    c = ops.make_packed([70, 60, 90], [400, 360, 390], 4, 2, hd, dt, seed=6)
+    want, tol = ops.ref_packed(c)
+    d = dict(c, **{x: c[x].copy() for x in "qkv"})
+    d["k"][c["ks"][1]:c["ks"][2]] = bad
+    d["v"][c["ks"][1]:c["ks"][2]] = bad
+    d["q"][c["qs"][1]:c["qs"][2]] = bad
+    got = run_packed(dev, d)
+    for i in (0, 2):
+        at = slice(c["qs"][i], c["qs"][i + 1])
+        ops.close(got[at], want[at], tol[at])
+    assert not np.isfinite(got[c["qs"][1]:c["qs"][2]]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("hd,dt", [(64, wk.BF16), (128, wk.F16)])
+@pytest.mark.parametrize("key", [137, 2580])
+def test_packed_non_finite_values_in_a_cluster(dev, bad, hd, dt, key):
+    """A NaN or an infinity in V where a cluster shares the keys: it reaches the queries that see its key, in its dimension."""
+    c = ops.make_packed([40], [2600], 2, 1, hd, dt, seed=8)
+    want, tol = ops.ref_packed(c)
+    d = dict(c, v=c["v"].copy())
+    d["v"][key, 3] = bad
+    got = run_packed(dev, d)
+    seen = np.zeros(want.shape, bool)
+    seen[max(key - 2560, 0):, [3, hd + 3]] = True
+    assert not np.isfinite(got[seen]).any()
+    assert (np.abs(got - want) <= tol)[~seen].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,hd", [(wk.F16, 64), (wk.BF16, 128)])
+def test_packed_long_context_with_rows_beyond_32_bits(dev, dt, hd):
+    """Rows so far apart that the last ones lie more than 2^32 bytes behind the first, in K, V, the queries and the output."""
+    c = ops.make_packed([40], [600], 2, 1, hd, dt, seed=3)
+    q_rs, k_rs = 1 << 26, 1 << 22
+    q, k, v, out = (alloc(2 * ((n - 1) * rs + w)) for n, rs, w in ((40, q_rs, 2 * hd), (600, k_rs, hd), (600, k_rs, hd),
+                                                                   (40, q_rs, 2 * hd)))
+    for p, x, rs in ((q, c["q"], q_rs), (k, c["k"], k_rs), (v, c["v"], k_rs)):
+        rows = to_bits(x, dt)
+        for r in range(len(x)):
+            dev.cuda_to_device(p + 2 * r * rs, ops.as_p(np.ascontiguousarray(rows[r])), rows[r].nbytes)
+    qs, ks = up(c["qs"].astype(np.int32)), up(c["ks"].astype(np.int32))
+    wk.check(dev.wk_attention_packed(out, q_rs, q, q_rs, k, k_rs, v, k_rs, qs, ks, 1, 40, 600, 2, 1, hd, dt))
+    got = ops.from_bits(np.stack([down(out + 2 * r * q_rs, 2 * hd, ops.RAW[dt]) for r in range(40)]), dt)
+    free(q, k, v, out, qs, ks)
+    want, tol = ops.ref_packed(c)
+    ops.close(got, want, tol)
