@@ -8,6 +8,9 @@ and the weights sum to at least one such: 2^-34 sum |v| of the keys that a row
 sees.  An output in fp16 is exact to 2^-25 at the least.
 """
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -353,3 +356,28 @@ def test_packed_long_context_with_rows_beyond_32_bits(dev, dt, hd):
     free(q, k, v, out, qs, ks)
     want, tol = ops.ref_packed(c)
     ops.close(got, want, tol)
+
+
+WITHOUT_TCGEN05 = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import numpy as np
+import wukong_b200 as wk
+from tests import test_serving_ops as ops
+L = wk.lib()
+L.cuda_init(0)
+for case in (([300, 1, 70], [700, 1, 70], 4, 2, 128, wk.F16), ([40], [2600], 2, 1, 64, wk.BF16),
+             ([50, 260], [50, 400], 130, 1, 64, wk.BF16), ([5] * 30 + [300], [5] * 30 + [300], 4, 2, 64, wk.F16)):
+    c = ops.make_packed(*case, seed=5)
+    want, tol = ops.ref_packed(c)
+    ops.close(ops.run_packed(L, c), want, tol)
+print("ok")
+"""
+
+
+@pytest.mark.gpu
+def test_packed_without_the_tcgen05_kernel():
+    """What serves where a compiler gave that kernel other registers than its split counts on."""
+    env = dict(os.environ, WUKONG_TC_ATTN="0")
+    r = subprocess.run([sys.executable, "-c", WITHOUT_TCGEN05, wk.ROOT], capture_output=True, text=True, env=env, timeout=300)
+    assert r.returncode == 0 and r.stdout.endswith("ok\n"), r.stdout + r.stderr

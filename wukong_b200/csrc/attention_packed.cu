@@ -1200,21 +1200,31 @@ bool pk_map(CUtensorMap *m, const void *base, int dtype, int D, int heads, int r
                          CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, const PkMaps &maps, int GT, cudaStream_t s) {
-    using L = PkLayout<D>;
-    constexpr size_t smem = L::kBars + sizeof(PkBars<D>) + 1024;
+// Sets the tcgen05 kernel up on the current device.  *fits: it has the registers that its split
+// counts on; where a compiler gave it others, the split would wait for registers that the launch
+// does not have, and the other kernels serve.
+template <typename T, int D> cudaError_t ready_packed(bool *fits) {
+    constexpr size_t smem = PkLayout<D>::kBars + sizeof(PkBars<D>) + 1024;
     static_assert(smem <= 232448, "shared memory of a CTA");
     auto kern = attn_packed_kernel<T, D>;
     static int configured = -1;  // the device that the kernel is set up for
+    static bool as_split = false;
     if (configured != g_rt.device) {
         cudaFuncAttributes fa;
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);
         if (e != cudaSuccess) return e;
-        if (fa.numRegs != kPkRegs) return cudaErrorInvalidKernelImage;  // the register split would not add up
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
+        as_split = fa.numRegs == kPkRegs;
         configured = g_rt.device;
     }
+    *fits = as_split && g_rt.tc_attn;
+    return cudaSuccess;
+}
+
+template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, const PkMaps &maps, int GT, cudaStream_t s) {
+    constexpr size_t smem = PkLayout<D>::kBars + sizeof(PkBars<D>) + 1024;
+    auto kern = attn_packed_kernel<T, D>;
     PkArgs a;
     a.out = p.out;
     a.out_rs = p.out_rs;
@@ -1349,8 +1359,9 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
     PackedArgs a{out, out_rs, q, k, v, q_rs, k_rs, v_rs, q_starts, k_starts, n, q_rows, k_rows, n_heads, kv_heads,
                  1.0f / sqrtf((float)head_dim), (uintptr_t)out % 4 == 0 && out_rs % 2 == 0, -1, n};
     cudaStream_t s = stream();
-    cudaError_t e;
+    cudaError_t e = cudaSuccess;
     // TMA wants 16-byte aligned bases and strides; what is not goes row by row
+    bool by_rows = true;
     const uintptr_t low = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v;
     if (low % 16 == 0 && (q_rs | k_rs | v_rs) % 8 == 0 && k_rows > 0) {
         const int G = n_heads / kv_heads, GT = G < 128 ? G : 128;
@@ -1371,13 +1382,26 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
         // base(n) of that kernel, with all rows
         long long units = (long long)q_rows * G / 64 + n;
         if (units > q_rows) units = q_rows;
-        const bool some_short = G <= 64 && units <= 65535 && kv_heads <= 65535 &&
-                                (n == 1 ? k_rows <= reach * 3 / 4 : k_rows <= reach || k_rows <= (long long)mean * n);
-        const bool some_long = !some_short || k_rows > reach;
+        const bool can_short = G <= 64 && units <= 65535 && kv_heads <= 65535;
+        bool some_short =
+            can_short && (n == 1 ? k_rows <= reach * 3 / 4 : k_rows <= reach || k_rows <= (long long)mean * n);
+        bool some_long = !some_short || k_rows > reach;
         const int longer = k_rows / (reach + 1);  // key rows are nobody's twice
         a.reach = some_short ? reach : -1;
         a.longer = some_short && longer < n ? longer : n;
-        e = cudaSuccess;
+        if (some_long) {
+            bool fits = false;
+            if (dtype == kF16)
+                e = head_dim == 64 ? ready_packed<__half, 64>(&fits) : ready_packed<__half, 128>(&fits);
+            else
+                e = head_dim == 64 ? ready_packed<__nv_bfloat16, 64>(&fits) : ready_packed<__nv_bfloat16, 128>(&fits);
+            if (e != cudaSuccess) return fail_cuda("wk_attention_packed", e);
+            if (!fits) {  // all are the short kernel's, or go row by row
+                some_long = false;
+                some_short = can_short;
+                a.reach = k_rows;
+            }
+        }
         if (some_long) {
             PkMaps maps;
             if (!pk_map(&maps.q, q, dtype, head_dim, n_heads, q_rows, q_rs, GT, 128 / GT) ||
@@ -1399,10 +1423,14 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
                 e = head_dim == 64 ? launch_short<__nv_bfloat16, 64>(a, (int)units, s)
                                    : launch_short<__nv_bfloat16, 128>(a, (int)units, s);
         }
-    } else if (dtype == kF16)
-        e = head_dim == 64 ? launch_rows<__half, 64>(a, s) : launch_rows<__half, 128>(a, s);
-    else
-        e = head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(a, s) : launch_rows<__nv_bfloat16, 128>(a, s);
+        by_rows = !some_long && !some_short;
+    }
+    if (by_rows) {
+        if (dtype == kF16)
+            e = head_dim == 64 ? launch_rows<__half, 64>(a, s) : launch_rows<__half, 128>(a, s);
+        else
+            e = head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(a, s) : launch_rows<__nv_bfloat16, 128>(a, s);
+    }
     if (e != cudaSuccess) return fail_cuda("wk_attention_packed", e);
     return 0;
 }

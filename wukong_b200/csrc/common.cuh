@@ -78,6 +78,7 @@ struct Runtime {
     size_t ws_size = 0;
     bool pdl = true;      // programmatic dependent launch on the hot kernels
     bool tc_gemm = true;  // tcgen05 GEMM for activation blocks of >= 16 rows
+    bool tc_attn = true;  // tcgen05 kernel of packed prompt attention
     int warp_tile_min = 4096;  // SwiGLU / logits layers with this many 16-row tiles run one tile per warp
     long l2_prefetch_max = 12L << 20;  // engine: bytes of the next layer's weights each linear layer prefetches into L2
     // limit of the cross-GPU flag waits of the tensor-parallel exchange

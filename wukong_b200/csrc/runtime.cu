@@ -91,6 +91,8 @@ void cuda_init(int idx) {
     g_rt.pdl = !(pdl && pdl[0] == '0');
     const char *tc = getenv("WUKONG_TC_GEMM");
     g_rt.tc_gemm = !(tc && tc[0] == '0');
+    const char *ta = getenv("WUKONG_TC_ATTN");
+    g_rt.tc_attn = !(ta && ta[0] == '0');
     const char *wt = getenv("WUKONG_WARP_TILE_MIN");
     if (wt && atoi(wt) > 0) g_rt.warp_tile_min = atoi(wt);
     const char *pfm = getenv("WUKONG_L2_PREFETCH_MB");
