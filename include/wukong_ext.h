@@ -116,8 +116,8 @@ int wk_attention_decode(void *out, const void *q, const void *kpool, const void 
 
 /* ---- Continuous batching over an 8-bit paged K/V cache (no counterpart in
  * the reference, which has no cache).  One step of a serving loop: wk_batch_plan
- * (the maps of the step), wk_attention_packed (prompts) or wk_kv8_attention
- * (single tokens), wk_kv8_store (append).  All run on the library stream, do not
+ * (the maps of the step), wk_kv8_store (append), wk_kv8_attention (tokens of running
+ * sequences) and wk_attention_packed (prompts that start).  All run on the library stream, do not
  * synchronise, allocate nothing and may be captured into a graph.  Each returns 0,
  * or -1 with the reason in wk_last_error() and nothing launched.
  *
@@ -127,7 +127,7 @@ int wk_attention_decode(void *out, const void *q, const void *kpool, const void 
  * page id outside [0, n_pages) stands for no page: a token stored there is
  * dropped, a key there is not attended to. */
 
-/* The maps of one step, from request lengths: sequence i (0 <= i < n <= 8192)
+/* The maps of one step, from request lengths: sequence i (0 <= i < n, n 1 to 8192)
  * has ctx[i] tokens in the cache and brings add[i] (0: none) more.  Device
  * arrays, negative lengths count as 0:
  *   starts [n + 1]  first packed row of each sequence; starts[n] is the row count
@@ -177,8 +177,10 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
  * q_starts[i] .. q_starts[i+1] - 1 and the key rows k_starts[i] .. k_starts[i+1] - 1
  * (device int [n + 1], ascending), and its queries are the last of its keys: query j
  * of Lq sees keys 0 .. Lk - Lq + j of its own sequence; one that sees none gets
- * zeros.  Starts beyond q_rows or k_rows count as q_rows or k_rows (a plan of more
- * rows than there is room for).  Rows outside every sequence are neither read nor written.  q / out
+ * zeros.  K and V are rows, not the cache: with the plan's starts for both, this is
+ * for sequences that start in the step (ctx 0).  Starts beyond q_rows or k_rows count
+ * as q_rows or k_rows (a plan of more rows than there is room for).  Rows outside every
+ * sequence are neither read nor written.  q / out
  * [q_rows][n_heads][head_dim], k / v [k_rows][kv_heads][head_dim] with row strides in
  * elements (the slices of fused q|k|v rows serve; q, k and v 16-byte aligned with
  * strides that are multiples of 8 take the tensor-core kernel, others a slow one);

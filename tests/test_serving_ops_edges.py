@@ -381,3 +381,85 @@ def test_packed_without_the_tcgen05_kernel():
     env = dict(os.environ, WUKONG_TC_ATTN="0")
     r = subprocess.run([sys.executable, "-c", WITHOUT_TCGEN05, wk.ROOT], capture_output=True, text=True, env=env, timeout=300)
     assert r.returncode == 0 and r.stdout.endswith("ok\n"), r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,dt", [(8, 2, 64, wk.F16), (8, 1, 128, wk.BF16)])
+@pytest.mark.parametrize("run,adds", [(3, [1, 1, 3, 90, 20, 1]), (0, [5, 64, 0, 130, 1, 63]), (6, [1, 2, 1, 1, 0, 1]),
+                                      (2, [1, 0, 300, 0, 7, 1])])
+def test_step_of_running_and_starting_sequences(dev, heads, kv, hd, dt, run, adds):
+    """Running sequences first, over the cache; those that start behind them, over their own rows."""
+    loop = ops.Loop(dev, 6, heads, kv, hd, dt, n_pages=40, max_pages=8, rows_cap=700, seed=run)
+    if run:
+        loop.inputs([70 + 9 * i if i < run else 0 for i in range(6)])
+        loop.launch(prompts=True)
+        loop.verify(prompts=True)
+    loop.inputs(adds)
+    d, n, w, ow = loop.d, loop.n, loop.w, heads * hd
+    run_rows = sum(adds[:run])
+    q, k, v = d["qkv"], d["qkv"] + 2 * ow, d["qkv"] + 2 * (heads + kv) * hd
+    loop.put("out", np.full((loop.rows_cap, ow), 0x3555, np.uint16))
+    wk.check(dev.wk_batch_plan(d["starts"], d["lens"], d["seq"], d["pos"], d["slot"], loop.rows_cap, d["table"],
+                               loop.max_pages, d["status"], d["ctx"], d["add"], n, d["free"], d["n_free"], loop.n_pages))
+    wk.check(dev.wk_kv8_store(d["k"], d["v"], d["ks"], d["vs"], loop.n_pages, k, w, v, w, d["starts"], d["ctx"], n,
+                              loop.rows_cap, d["table"], loop.max_pages, kv, hd, dt))
+    wk.check(dev.wk_kv8_attention(d["out"], ow, q, w, d["k"], d["v"], d["ks"], d["vs"], loop.n_pages, d["table"], n,
+                                  loop.max_pages, d["seq"], d["pos"], run_rows, loop.max_pages * PAGE, heads, kv, hd, dt,
+                                  d["ws"], loop.ws_bytes))
+    wk.check(dev.wk_attention_packed(d["out"], ow, q, w, k, w, v, w, d["starts"] + 4 * run, d["starts"] + 4 * run, n - run,
+                                     loop.rows_cap, loop.rows_cap, heads, kv, hd, dt))
+    out = down(d["out"], (loop.rows_cap, ow), ops.RAW[dt])
+    p = ops.ref_plan(loop.ctx, loop.add, loop.table, np.roll(loop.free_list, -loop.taken), loop.n_pages - loop.taken,
+                     loop.rows_cap)
+    rows = len(loop.x)
+    for i in range(2):
+        x = loop.x[:, ow + i * kv * hd:ow + (i + 1) * kv * hd].reshape(rows, kv, hd)
+        loop.codes[i], loop.scales[i] = ops.ref_store(loop.codes[i], loop.scales[i], x, p["starts"], loop.ctx, p["table"],
+                                                      loop.n_pages)
+    c = dict(heads=heads, kv=kv, hd=hd, dt=dt, q=loop.x[:, :ow])
+    over_cache = ops.ref_decode(dict(c, pos=p["row_pos"][:rows], seq=p["row_seq"][:rows], table=p["table"],
+                                     codes=loop.codes, scales=loop.scales, n_pages=loop.n_pages))
+    over_rows = ops.ref_packed(dict(c, k=loop.x[:, ow:ow + kv * hd], v=loop.x[:, ow + kv * hd:], qs=p["starts"], ks=p["starts"]))
+    want, tol = (np.concatenate([a[:run_rows], b[run_rows:]]) for a, b in zip(over_cache, over_rows))
+    ops.close(ops.from_bits(out[:rows], dt), want, tol)
+    assert (out[rows:].view(np.uint16) == 0x3555).all()
+    loop.end()
+
+
+CAPTURED_FIRST = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import numpy as np
+import torch
+import wukong_b200 as wk
+from tests import test_serving_ops as ops
+L = wk.lib()
+L.cuda_init(0)
+stream = torch.cuda.ExternalStream(L.wk_stream())
+loop = ops.Loop(L, 4, 8, 2, 128, wk.F16, 80, 16, 900, seed=2)
+loop.inputs([20, 700, 1, 64])
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=stream):
+    loop.launch(prompts=True)
+with torch.cuda.stream(stream):
+    g.replay()
+loop.verify(prompts=True)
+loop.inputs([1, 1, 0, 5])
+g2 = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g2, stream=stream):
+    loop.launch(prompts=False)
+with torch.cuda.stream(stream):
+    g2.replay()
+loop.verify(prompts=False)
+torch.cuda.synchronize()
+print("ok")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_captured():
+    """Kernels that are set up within a capture."""
+    pytest.importorskip("torch")
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST, wk.ROOT], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.endswith("ok\n"), r.stdout + r.stderr

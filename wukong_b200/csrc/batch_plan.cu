@@ -8,8 +8,9 @@
 //   table[i][have_i + j] = free[base_i + j]        for the need_i - have_i new pages
 //   row r of sequence i: pos = ctx_i + r - starts_i, slot = 64 table[i][pos / 64] + pos % 64
 //
-// The outputs are a few hundred kilobytes at most, so latency bounds the
-// kernel: one launch, and every CTA computes the prefix sums of all sequences
+// A step writes 16 bytes for each row of rows_cap, the -1 behind the last row
+// included (117 KB for 7.3 k rows), so latency bounds it unless rows_cap is far
+// beyond the step: one launch, and every CTA computes the prefix sums of all sequences
 // itself (8 bytes each, from L2) instead of waiting for another CTA.  A row
 // reads table entries below have_i only, and the launch writes entries from
 // have_i on only, so the CTAs need no order among themselves.  A step of 64
