@@ -415,8 +415,8 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
 // which the tensor cores run 2048 and the exponentials fill their pipe for 2048;
 // the two overlap except where S, P and the barriers between them change hands
 // (a barrier's answer waits 150 to 350 cycles behind queued exponentials).  8192 x 32
-// heads of 128 over 8: 440 us, 1250 TFLOP/s; behind a long context the tensor pipe is
-// active 62 % of the time.  Measured and not kept: exponentials on the FMA pipe by
+// heads of 128 over 8: 454 us or 1210 TFLOP/s by itself, 510 to 520 us in calls over
+// seconds, under the power cap; behind a long context the tensor pipe is active 61 % of the time.  Measured and not kept: exponentials on the FMA pipe by
 // a polynomial for 1/8 to 1/2 of the keys (no faster), an issuing warp per tile (the
 // tiles fall in phase, 16 % slower), P in TMEM columns of its own for D = 64 (the same
 // time), one tile per CTA and two CTAs per SM (25 % slower at 8192), persistent
@@ -1020,10 +1020,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     m = __fsub_ru(m, a.shift);
                 }
                 half(0, true, m, sum, pv);
-                const float mb = pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                const bool move = (mb - m) * a.scale_log2 > PkWeight<T>::lead + PkWeight<T>::bias || (m == -INFINITY && mb > m);
+                const float mb = __fsub_ru(pk_max3(pk_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), a.shift);
+                const bool move = (mb - m) * a.scale_log2 > PkWeight<T>::lead || (m == -INFINITY && mb > m);
                 if (__any_sync(0xffffffffu, move)) {
-                    const float mn = move ? __fsub_ru(mb, a.shift) : m;
+                    const float mn = move ? mb : m;
                     const float f = mn == m || m == -INFINITY ? 1.f : pk_ex2((m - mn) * a.scale_log2);
                     m = mn;
                     l *= f;
@@ -1282,7 +1282,7 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     long long split = blocks / 2 < g_rt.num_sms / ctas ? (long long)(blocks / 2) : g_rt.num_sms / ctas;
     if (split > 8) split = 8;
     // (of one sequence the units are exact; of several they are fewer than `units`, which leaves room)
-    while (n == 1 && split > 1 && at_once[split] < ctas) --split;
+    while (split > 1 && at_once[split] < (n == 1 ? ctas : 1)) --split;
     const double full = (double)p.q_rows / ((double)n * 2 * PT);  // how full units are, on average
     const double join = 2 + (full < 1 ? full : 1) * ((D == 64 ? 1 : 3) + (split < 4 ? D / 64 : 0));  // in blocks
     const double longer = n > 2 ? 1.5 : 1;  // of several, the longest ends last
@@ -1367,27 +1367,29 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
         const int G = n_heads / kv_heads, GT = G < 128 ? G : 128;
         // Short sequences go to the kernel for them.  The host knows room and count only, and idle
         // sequences and room without rows hide a long one; so where all of them may be short but one
-        // could have more than `reach` keys, both kernels are launched and each takes its own sequences
-        // by their lengths.  A sequence by itself and short ones throughout, us, short kernel / tcgen05 /
-        // both, 32 / 8 heads of 128:
-        //   1 of 192           9.6 / 10.1         24 of 16     7.5 / 15.1 /  8.9    100 of 16  15.1 / 44.1 / 19.0
-        //   1 of 256          11.6 / 10.2         24 of 60    14.8 / 17.2 / 18.4    100 of 40  36.8 / 55.0 / 45.4
-        //   1 of 4096, 63 of 0  452 / 127 / 129   24 of 97    26.6 / 26.2           400 of 40   144 /  231 /  182
+        // could be long, both kernels are launched and each takes its own sequences by their lengths.
+        // The second launch takes the host 2 us, so up to `alone` keys in all the short kernel serves
+        // alone.  us, short kernel / tcgen05 / both, 32 / 8 heads of 128:
+        //   1 of 192             9.6 / 10.1         24 of 16     7.4 / 15.0         100 of 16  15.0 / 44.1 / 19.0
+        //   1 of 256            11.6 / 10.2         24 of 40    13.0 / 17.3 / 14.9  100 of 40  36.8 / 55.1 / 45.4
+        //   512 and 63 of 0     26.8 / 13.9         24 of 60    14.8 / 17.3 / 18.4  400 of 40   144 /  231 /  182
+        //   4096 and 63 of 0     452 /  127 /  129  24 of 97    26.6 / 26.3
         // 16 / 4 heads of 64:
-        //   1 of 384           9.5 / 10.2         24 of 40     5.6 /  7.4 /  7.6    100 of 40  11.7 / 22.7 / 15.7
-        //   1 of 768          17.3 / 16.8         24 of 97    10.1 / 14.0 / 13.4    400 of 97   109 /  175 /  150
-        //   1 of 4096, 63 of 0  134 /  59 /  61   24 of 200   16.9 / 20.7
+        //   1 of 384             9.5 / 10.2         24 of 40     5.5 /  7.4         100 of 40  11.7 / 22.7 / 15.7
+        //   1 of 768            17.3 / 16.8         24 of 97    10.1 / 14.0 / 13.4  400 of 97   109 /  175 /  150
+        //   4096 and 63 of 0     134 /   59 /   60  24 of 200   16.9 / 20.7
         const int reach = head_dim == 64 ? 512 : 256;
+        const int alone = head_dim == 64 ? 640 : 512;
         const int mean = head_dim == 64 ? 112 : 48;
         // base(n) of that kernel, with all rows
         long long units = (long long)q_rows * G / 64 + n;
         if (units > q_rows) units = q_rows;
         const bool can_short = G <= 64 && units <= 65535 && kv_heads <= 65535;
         bool some_short =
-            can_short && (n == 1 ? k_rows <= reach * 3 / 4 : k_rows <= reach || k_rows <= (long long)mean * n);
-        bool some_long = !some_short || k_rows > reach;
+            can_short && (n == 1 ? k_rows <= reach * 3 / 4 : k_rows <= alone || k_rows <= (long long)mean * n);
+        bool some_long = !some_short || k_rows > alone;
         const int longer = k_rows / (reach + 1);  // key rows are nobody's twice
-        a.reach = some_short ? reach : -1;
+        a.reach = !some_short ? -1 : some_long ? reach : k_rows;
         a.longer = some_short && longer < n ? longer : n;
         if (some_long) {
             bool fits = false;

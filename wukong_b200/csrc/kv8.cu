@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(256, 6) kv8_store_kernel(Kv8Store a) {
 //   S^T[keys x heads] = K Q^T    m16n8k16, keys in M, 8 heads in N
 //   P   = exp2(c (S s_k - m) + 11)    m moves only when it is 2^4 behind
 //   O^T[dims x heads] += s_v (V^T P)
-// The cache is read once, straight into the registers that hold the A operands:
+// The cache is read once (by up to 16 heads per K/V head; more are several CTAs, each of which
+// reads it), straight into the registers that hold the A operands:
 // the contraction of Q K^T runs over dims in the order in which 16-byte pieces of
 // a K row fall to the four lanes of a row group, and V^T is formed from the bytes of four
 // keys by permutes, so no shared memory and no barrier stands between HBM and
