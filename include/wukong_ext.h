@@ -186,7 +186,7 @@ int wk_kv8_attention(void *out, long out_rs, const void *q, long q_rs, const voi
  * strides that are multiples of 8 take the tensor-core kernel, others a slow one);
  * n_heads a multiple of kv_heads, head_dim 64 or 128, dtype F16 or BF16.  A NaN or an
  * infinity in K or V reaches the queries that see its key, and no other (an
- * infinity in V may come out as a NaN). */
+ * infinity in V may come out as a NaN).  Scores |q . k| / sqrt(head_dim) up to 10^8. */
 int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const void *k, long k_rs, const void *v,
                         long v_rs, const int *q_starts, const int *k_starts, int n, int q_rows, int k_rows,
                         int n_heads, int kv_heads, int head_dim, int dtype);

@@ -111,7 +111,8 @@ __global__ void __launch_bounds__(128) attn_packed_rows_kernel(PackedArgs a) {
 // Blocks of 64 keys come through two stages of cp.async.  The contraction of Q K^T runs
 // over dims in the order in which 16-byte pieces of a row fall to the four lanes
 // of a row group, so Q goes from global memory straight into its fragments and a K
-// fragment is one 16-byte read.  m is the running maximum itself, so b = lead + bias: 15 in fp16, -24 in bf16.
+// fragment is one 16-byte read.  m is the running maximum itself, so b = lead + bias: 15 in
+// fp16, -24 in bf16.
 // Latency bounds it: unit -> Q, K, V -> S -> softmax -> O.  Small CTAs, several to an SM, and
 // no tensor memory, barriers or maps to set up are what it has over the tcgen05 kernel: 100
 // sequences of 40 tokens, 16 / 4 heads of 64, take 10.5 us instead of 22.0.  A further block
@@ -416,11 +417,12 @@ __global__ void __launch_bounds__(128, D == 128 ? 3 : 4) attn_packed_short_kerne
 // the two overlap except where S, P and the barriers between them change hands
 // (a barrier's answer waits 150 to 350 cycles behind queued exponentials).  8192 x 32
 // heads of 128 over 8: 454 us or 1210 TFLOP/s by itself, 510 to 520 us in calls over
-// seconds, under the power cap; behind a long context the tensor pipe is active 61 % of the time.  Measured and not kept: exponentials on the FMA pipe by
-// a polynomial for 1/8 to 1/2 of the keys (no faster), an issuing warp per tile (the
-// tiles fall in phase, 16 % slower), P in TMEM columns of its own for D = 64 (the same
-// time), one tile per CTA and two CTAs per SM (25 % slower at 8192), persistent
-// CTAs over units (24 ragged prompts 5 % faster, one of 8192 3 % slower).
+// seconds, under the power cap; behind a long context the tensor pipe is active 61 % of
+// the time.  Measured and not kept: exponentials on the FMA pipe by a polynomial for 1/8
+// to 1/2 of the keys (no faster), an issuing warp per tile (the tiles fall in phase, 16 %
+// slower), P in TMEM columns of its own for D = 64 (the same time), one tile per CTA and
+// two CTAs per SM (25 % slower at 8192), persistent CTAs over units (24 ragged prompts
+// 5 % faster, one of 8192 3 % slower).
 constexpr int kPkThreads = 384;
 constexpr int kPkRegs = 168;  // registers per thread at launch
 constexpr int kPkKeys = 128;  // keys per block
@@ -1263,8 +1265,8 @@ template <typename T, int D> cudaError_t launch_packed(const PackedArgs &p, cons
     cfg.attrs = attr;
     // Few units and long sequences: a cluster to each, where all run at once and it saves more
     // blocks of keys (of the mean length) than its join takes: 11 us with 2 or 3 CTAs, 8 us
-    // with more, heads of 64 7 and 5 us, 3 us where a unit has a row or two, a block taking 1.6.  8 heads of 128 over 1, us without / with
-    // 2 / 4 / 8 CTAs to a unit:
+    // with more, heads of 64 7 and 5 us, 3 us where a unit has a row or two, a block taking
+    // 1.6.  8 heads of 128 over 1, us without / with 2 / 4 / 8 CTAs to a unit:
     //   512 rows  13.8 / 21.7 / 16.5 / 30.0 (16 clusters of 8 do not fit)   500 behind 4000  67 / 48 / 30 / 40
     //   1024      20.6 / 25.2 / 18.3 / -     2048  34.1 / 32.6 / - / -      2000 behind 14000  216 / 126 / - / -
     static int at_once[9], at_once_on = -1;  // clusters of a size that run at once, on which device
@@ -1369,7 +1371,8 @@ int wk_attention_packed(void *out, long out_rs, const void *q, long q_rs, const 
         // sequences and room without rows hide a long one; so where all of them may be short but one
         // could be long, both kernels are launched and each takes its own sequences by their lengths.
         // The second launch takes the host 2 us, so up to `alone` keys in all the short kernel serves
-        // alone.  us, short kernel / tcgen05 / both, 32 / 8 heads of 128:
+        // alone; above `mean`, both take no less than the tcgen05 kernel alone.  us, short kernel /
+        // tcgen05 / both, 32 / 8 heads of 128:
         //   1 of 192             9.6 / 10.1         24 of 16     7.4 / 15.0         100 of 16  15.0 / 44.1 / 19.0
         //   1 of 256            11.6 / 10.2         24 of 40    13.0 / 17.3 / 14.9  100 of 40  36.8 / 55.1 / 45.4
         //   512 and 63 of 0     26.8 / 13.9         24 of 60    14.8 / 17.3 / 18.4  400 of 40   144 /  231 /  182
